@@ -20,7 +20,8 @@ OBJ = PKG / "_build"
 LIB = PKG / "libfpt_b200.so"
 COMPAT_LIB = PKG / "libfpt_b200_compat.so"          # the reference's launch_* names over the fpt_* C ABI
 COMPAT_SRC = CSRC / "fpt_compat_launch.cpp"
-TORCH_BINDING_SRC = CSRC / "fpt_torch_binding.cpp"   # compiled PyTorch binding of the hot element-wise operators
+# compiled PyTorch binding of the hot element-wise operators and of the operators around the attention
+TORCH_BINDING_SRCS = [CSRC / "fpt_torch_binding.cpp", CSRC / "fpt_torch_block.cpp"]
 TORCH_BINDING_NAME = "_fpt_torch"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xptxas", "-v",
@@ -106,19 +107,31 @@ def _build_torch_binding(force: bool, verbose: bool) -> Path:
     import torch
     from torch.utils import cpp_extension
     out = torch_binding_path()
-    deps = [TORCH_BINDING_SRC, LIB, PKG.parent / "include" / "fpt_b200.h"]
+    deps = [*TORCH_BINDING_SRCS, LIB, PKG.parent / "include" / "fpt_b200.h"]
     if force or _stale(out, deps):
         cuda_home = Path(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc").resolve().parents[1]
         includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], str(cuda_home / "include")]
         libdirs = cpp_extension.library_paths()
-        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-DTORCH_EXTENSION_NAME={TORCH_BINDING_NAME}",
-               "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-               *[f"-I{i}" for i in includes], str(TORCH_BINDING_SRC), "-o", str(out),
+        flags = ["-O2", "-std=c++17", "-fPIC", "-w", f"-DTORCH_EXTENSION_NAME={TORCH_BINDING_NAME}",
+                 "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                 *[f"-I{i}" for i in includes]]
+
+        def compile_one(src: Path) -> Path:
+            obj = OBJ / (src.stem + ".o")
+            if force or _stale(obj, [src, PKG.parent / "include" / "fpt_b200.h"]):
+                proc = subprocess.run(["g++", *flags, "-c", str(src), "-o", str(obj)], capture_output=True, text=True)
+                if proc.returncode != 0:
+                    raise RuntimeError(f"torch binding build failed for {src.name}:\n{proc.stderr[-4000:]}")
+            return obj
+
+        with ThreadPoolExecutor(max_workers=len(TORCH_BINDING_SRCS)) as pool:
+            objs = list(pool.map(compile_one, TORCH_BINDING_SRCS))
+        cmd = ["g++", "-shared", *map(str, objs), "-o", str(out),
                *[f"-L{d}" for d in libdirs], "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python",
                f"-L{PKG}", "-lfpt_b200", "-Wl,-rpath,$ORIGIN", *[f"-Wl,-rpath,{d}" for d in libdirs]]
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
-            raise RuntimeError(f"torch binding build failed:\n{proc.stderr[-4000:]}")
+            raise RuntimeError(f"torch binding link failed:\n{proc.stderr[-4000:]}")
         if verbose:
             print(f"built {out}")
     return out

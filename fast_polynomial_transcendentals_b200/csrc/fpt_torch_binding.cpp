@@ -18,6 +18,8 @@
 
 #include "../../include/fpt_b200.h"
 
+void register_block_operators(pybind11::module_& m);   // fpt_torch_block.cpp
+
 namespace {
 
 const char* const kFunctionNames[] = {"sigmoid", "tanh", "swish", "erf", "gelu"};
@@ -186,4 +188,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("swish_mul_bwd", &swish_mul_bwd);
     m.def("swish_mul_packed", &swish_mul_packed);
     m.def("swish_mul_packed_bwd", &swish_mul_packed_bwd);
+    register_block_operators(m);
 }

@@ -96,3 +96,10 @@ def rope_phase_increments(head_dim: int, theta: float = 500000.0, device=None) -
     inc = torch.round(freqs * (2.0 ** 32) / (2.0 * math.pi)).to(torch.int64)
     inc = torch.where(inc >= 2 ** 31, inc - 2 ** 32, inc).to(torch.int32)
     return inc if device is None else inc.to(device)
+
+
+def rope_axis_phase_increments(sections, theta: float = 10000.0, device=None) -> torch.Tensor:
+    """int32 Q0.32 phase increments for positions on several axes (`qk_rope.rope_axes`, blocked sections) where every axis
+    has frequencies of its own: section n starts anew, round(theta^(-i/n) * 2^32 / 2pi) for i = 0 .. n - 1.  For one
+    series of frequencies over all pairs use `rope_phase_increments`."""
+    return torch.cat([rope_phase_increments(2 * int(n), theta, device) for n in sections])

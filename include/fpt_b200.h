@@ -44,6 +44,7 @@ typedef struct CUstream_st* fpt_stream_t; /* == cudaStream_t */
 #define FPT_ERR_SCRATCH_TOO_SMALL (-9) /* the problem needs more than the library's fixed scratch array holds */
 
 enum { FPT_FP16 = 0, FPT_BF16 = 1 };
+enum { FPT_FP32 = 2 }; /* fpt_qk_rope and its backward pass, and weights and biases where a comment says so */
 enum { FPT_SRC_CURRENT = 0, FPT_SRC_SOLLYA = 1 };
 enum { FPT_FN_SIGMOID = 0, FPT_FN_TANH = 1, FPT_FN_SWISH = 2, FPT_FN_ERF = 3, FPT_FN_GELU = 4 };
 enum { FPT_FWD = 0, FPT_BWD = 1 };
@@ -357,6 +358,41 @@ int fpt_attention_bwd_routed(void* dq, void* dk, void* dv, const void* dout, con
                              const int64_t* k_strides, const int64_t* v_strides, const int64_t* out_strides,
                              const int64_t* dout_strides, int mode, int causal, float scale, float softcap, int log2_n,
                              int softcap_grad, int exp2_emu_backend, int exp2_emu_freq, void* status, fpt_stream_t stream);
+
+/* ---- queries and keys on their way into the attention: the root-mean-square norm of every head and the position rotation in
+ *      one pass, and the rotation alone with positions on several axes (no counterpart in the reference, whose fused RoPE,
+ *      fpt_rope_apply, rotates by 0 .. seq - 1 in fp16 arithmetic and has no gradient).
+ *          u = x / sqrt(mean(x^2) + eps),   y = R (weight * u)
+ *      q, k: [batch, seq, heads, head_dim] by their three outer strides in elements (batch, seq, head; head_dim
+ *      contiguous; any alignment, 16-byte rows are faster); q_out, k_out: contiguous, 16-byte aligned, of the same shape;
+ *      either side may have no heads.  dtype FPT_FP16, FPT_BF16 or FPT_FP32; weights [head_dim] of weight_dtype, or null
+ *      for ones.  Arithmetic is fp32, rounded once.
+ *      head_dim: a multiple of 8 up to 256.  pairs: a multiple of 4, 2 pairs <= head_dim; dimensions from 2 pairs on pass
+ *      through.  pairing: FPT_PAIRS_ADJACENT rotates (2i, 2i + 1) as fpt_rope_apply does, FPT_PAIRS_HALVES (i, i + pairs).
+ *      Pair i turns by (position * phase_increments[i] mod 2^32) / 2^32 of a circle.  positions: device, int32 or int64
+ *      (position_bits 32 or 64) at axis * strides[0] + batch * strides[1] + seq * strides[2] elements, or null for
+ *      0 .. seq - 1; pair_axes: HOST array of `pairs` axis numbers below 4, read before the call returns, or null for
+ *      axis 0 throughout.  The caller answers for positions having that many axes.
+ *      norm 0: the rotation alone (weights and eps unused); inverse 1 then rotates backwards, which is the gradient. */
+enum { FPT_PAIRS_ADJACENT = 0, FPT_PAIRS_HALVES = 1 };
+int fpt_qk_rope(void* q_out, void* k_out, const void* q, const void* k, const void* q_weight, const void* k_weight,
+                const void* phase_increments, const void* positions, int position_bits, const int64_t* position_strides,
+                const uint8_t* pair_axes, int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads, int64_t head_dim,
+                int64_t pairs, const int64_t* q_strides, const int64_t* k_strides, int pairing, int norm, float eps,
+                int inverse, int dtype, int weight_dtype, fpt_stream_t stream);
+/* Its gradient with the norm, from q and k themselves (nothing is kept by the forward pass): dq, dk contiguous and 16-byte
+ *      aligned; dq_weight, dk_weight [head_dim] of weight_dtype, or null where not wanted.  dq_out, dk_out by strides.
+ *      workspace (device, 4-byte aligned, fpt_qk_norm_rope_bwd_workspace_bytes on the current device): the blocks' partial
+ *      weight gradients, summed in a fixed order; the call owns it until its work on `stream` has finished. */
+int64_t fpt_qk_norm_rope_bwd_workspace_bytes(int64_t q_heads, int64_t k_heads, int64_t head_dim);
+int fpt_qk_norm_rope_bwd(void* dq, void* dk, void* dq_weight, void* dk_weight, const void* dq_out, const void* dk_out,
+                         const void* q, const void* k, const void* q_weight, const void* k_weight,
+                         const void* phase_increments, const void* positions, int position_bits,
+                         const int64_t* position_strides, const uint8_t* pair_axes, void* workspace,
+                         int64_t workspace_bytes, int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads,
+                         int64_t head_dim, int64_t pairs, const int64_t* q_strides, const int64_t* k_strides,
+                         const int64_t* dq_out_strides, const int64_t* dk_out_strides, int pairing, float eps, int dtype,
+                         int weight_dtype, fpt_stream_t stream);
 
 /* ---- diagnostic: one 128x128x128 bf16 tile through the tensor-core building blocks of the attention kernel
  *      (no counterpart in the reference).  a, b: bf16 [128,128] row-major; c: fp32 [128,128];
