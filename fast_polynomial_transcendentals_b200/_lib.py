@@ -54,6 +54,11 @@ SIGNATURES: dict[str, list] = {
     "fpt_qk_norm_rope_bwd_workspace_bytes": [_i64, _i64, _i64],
     "fpt_qk_norm_rope_bwd": [_vp] * 12 + [_int, ctypes.POINTER(_i64), ctypes.c_char_p, _vp] + [_i64] * 7 +
                             [ctypes.POINTER(_i64)] * 4 + [_int, ctypes.c_float, _int, _int, _vp],
+    "fpt_linear": [_vp] * 6 + [_i64] * 8 + [_int] * 5 + [_vp, _vp],
+    "fpt_linear_grad_act_workspace_bytes": [_i64, _i64],
+    "fpt_linear_grad_act": [_vp] * 5 + [_i64] * 6 + [_int, _int, _vp],
+    "fpt_linear_grad_input": [_vp] * 3 + [_i64] * 6 + [_int, _vp, _vp],
+    "fpt_linear_grad_weight": [_vp] * 3 + [_i64] * 6 + [_int, _vp, _vp],
     "fpt_attention_fwd": [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, ctypes.POINTER(_i64), ctypes.POINTER(_i64),
                           ctypes.POINTER(_i64), ctypes.POINTER(_i64), _int, _int, ctypes.c_float, ctypes.c_float, _int, _vp, _vp],
     "fpt_attention_bwd_workspace_bytes": [_i64, _i64, _i64],
@@ -78,7 +83,7 @@ SIGNATURES: dict[str, list] = {
 _RESTYPES = {"fpt_status_string": ctypes.c_char_p, "fpt_version": ctypes.c_char_p,
              "fpt_rope_static_table_capacity": ctypes.c_int64, "fpt_attention_bwd_workspace_bytes": ctypes.c_int64,
              "fpt_attention_bwd_fused_workspace_bytes": ctypes.c_int64,
-             "fpt_qk_norm_rope_bwd_workspace_bytes": ctypes.c_int64}
+             "fpt_qk_norm_rope_bwd_workspace_bytes": ctypes.c_int64, "fpt_linear_grad_act_workspace_bytes": ctypes.c_int64}
 SIGNATURES["fpt_status_string"] = [_int]
 SIGNATURES["fpt_version"] = []
 

@@ -33,6 +33,8 @@ int tuning_gate_up_cta_pair();      // gate / up projection on pairs of CTAs (ct
 int tuning_attention_cta_pair();    // attention forward on pairs of CTAs (cta_group::2) where two blocks share their K / V: 0 never, 1 where possible
 int tuning_gate_up_tile_rows();     // gate / up projection: rows per tile, 128 or 256 (0: 256 for dense, 128 for grouped problems)
 int tuning_rope_heads_per_block();   // fused RoPE: heads one block rotates (0: all of them)
+int tuning_linear_tokens();      // linear layer: tokens per tile of the few-row form (16, 32, 64, 128), 0 the pair form, -1 (default) by size
+int tuning_linear_split();       // linear layer, few-row form: blocks that share an output tile along K, 0 (default) by size
 int tuning_attention_split();    // attention forward, column-split score-mod warps: 0 never, 1 soft-capped mode (default), 2 sigmoid mode too
 
 inline int cuda_status(cudaError_t e) { return e == cudaSuccess ? FPT_OK : int(e); }

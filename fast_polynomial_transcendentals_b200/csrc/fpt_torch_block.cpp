@@ -3,6 +3,9 @@
 //
 //   fpt_b200::qk_rope            norm of every head and rotation, or the rotation alone (fpt_qk_rope)
 //   fpt_b200::qk_norm_rope_bwd   gradient of the form with the norm
+//   fpt_b200::linear_act         act(x W^T + b) + r (fpt_linear)
+//   fpt_b200::linear_act_slope   the same with act' beside it, what a training step keeps
+//   fpt_b200::linear_act_bwd     its gradient (fpt_linear_grad_act, _grad_input, _grad_weight)
 //
 // The Python module enters through plain functions that check the arguments that are not tensors and call the dispatcher
 // (an eager call costs no boxing); graphs use torch.ops.fpt_b200.  Gradients are registered here as well: the backward
@@ -255,7 +258,236 @@ std::tuple<Tensor, Tensor> qk_rope_autograd(const Tensor& q, const Tensor& k, co
     return {out[0], out[1]};
 }
 
-// the eager door: off the GPU the checks run here, where no kernel would be found
+// ---- fpt_linear -----------------------------------------------------------------------------------------------------
+
+// The word a bounded device-side wait reports to: mapped host memory, so that a call looks at it without a copy or an
+// event.  One for the process, made at the first call (also inside a stream capture, where plain allocation is an error).
+volatile uint32_t* status_word() {
+    static uint32_t* word = [] {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        void* p = nullptr;
+        const cudaError_t e = cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        TORCH_CHECK(e == cudaSuccess, "no host memory for the status word: ", cudaGetErrorString(e));
+        *static_cast<uint32_t*>(p) = 0;
+        return static_cast<uint32_t*>(p);
+    }();
+    return word;
+}
+
+void poll_linear_status() {
+    volatile uint32_t* word = status_word();
+    const uint32_t value = *word;
+    if (value) {
+        *word = 0;
+        TORCH_CHECK(false, fpt_status_string(FPT_ERR_DEVICE_TIMEOUT), ": status word ", value, " (waiting point ", value & 0xffff,
+                    ") left by an earlier linear_act; the outputs of that call are invalid");
+    }
+}
+
+struct Linear {
+    int64_t rows, dim, out;
+    std::vector<int64_t> shape;         // of the result
+};
+
+Linear check_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int64_t function,
+                    int64_t degree, int64_t source) {
+    TORCH_CHECK(x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16, "x must be float16 or bfloat16");
+    TORCH_CHECK(weight.scalar_type() == x.scalar_type(), "x and weight must have the same dtype");
+    TORCH_CHECK(x.dim() >= 1 && weight.dim() == 2, "x must be [..., dim] and weight [out, dim]");
+    Linear l;
+    l.dim = weight.size(1), l.out = weight.size(0);
+    TORCH_CHECK(x.size(-1) == l.dim, "x has ", x.size(-1), " columns, the weight wants ", l.dim);
+    TORCH_CHECK(l.dim > 0 && l.dim % 8 == 0, "dim must be a positive multiple of 8");
+    TORCH_CHECK(l.out > 0, "weight must have at least one row");
+    l.rows = x.numel() / l.dim;
+    l.shape = x.sizes().vec();
+    l.shape.back() = l.out;
+    if (bias)
+        TORCH_CHECK(floating(*bias) && bias->dim() == 1 && bias->numel() == l.out, "bias must be a float16, bfloat16 or float32 tensor of ", l.out, " entries");
+    if (residual) {
+        TORCH_CHECK(residual->scalar_type() == x.scalar_type(), "x and residual must have the same dtype");
+        TORCH_CHECK(residual->sizes() == at::IntArrayRef(l.shape), "residual must have the shape of the result");
+    }
+    TORCH_CHECK(function >= FPT_FN_NONE && function <= FPT_FN_GELU && function != FPT_FN_ERF, "unknown activation");
+    TORCH_CHECK(degree == 0 || (degree >= 3 && degree <= 6 && function != FPT_FN_NONE), "Unsupported degree: ", degree);
+    TORCH_CHECK(source == 0 || (source == 1 && x.scalar_type() == at::kBFloat16), "FP16 spline kernels only support coeff_source=current");
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    for (const Tensor& t : {weight, bias.value_or(x), residual.value_or(x)})
+        TORCH_CHECK(t.device() == x.device(), "all tensors must be on the CUDA device of x");
+    return l;
+}
+
+int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// [rows, columns] with contiguous rows that do not overlap
+Tensor as_rows(const Tensor& t, int64_t rows, int64_t columns) {
+    Tensor r = t.reshape({rows, columns});
+    if ((columns > 1 && r.stride(1) != 1) || (rows > 1 && r.stride(0) < columns)) r = r.contiguous();
+    return r;
+}
+bool loadable(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && row_stride(t) % 8 == 0; }
+// the same as a matrix operand: rows on 16-byte boundaries
+Tensor as_operand(const Tensor& t, int64_t rows, int64_t columns) {
+    Tensor r = as_rows(t, rows, columns);
+    return loadable(r) ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+
+std::tuple<Tensor, Tensor> run_linear(const Tensor& x_in, const Tensor& weight_in, const OptTensor& bias_in, const OptTensor& residual_in,
+                                      int64_t function, int64_t degree, int64_t source, bool want_slope) {
+    const Linear l = check_linear(x_in, weight_in, bias_in, residual_in, function, degree, source);
+    poll_linear_status();
+    const c10::cuda::CUDAGuard guard(x_in.device());
+    Tensor out = at::empty(l.shape, x_in.options(), at::MemoryFormat::Contiguous);
+    const int64_t padded = (l.out + 7) / 8 * 8;
+    Tensor slope = at::empty({want_slope && function != FPT_FN_NONE ? l.rows : 0, padded}, x_in.options().dtype(at::kHalf), at::MemoryFormat::Contiguous);
+    if (l.rows == 0) return {out, slope};
+    const Tensor x = as_operand(x_in, l.rows, l.dim), weight = as_operand(weight_in, l.out, l.dim);
+    const Tensor bias = bias_in ? bias_in->contiguous() : Tensor();
+    const Tensor residual = residual_in ? as_rows(*residual_in, l.rows, l.out) : Tensor();
+    const int rc = fpt_linear(out.data_ptr(), slope.numel() ? slope.data_ptr() : nullptr, x.data_ptr(), weight.data_ptr(),
+                              bias.defined() ? bias.data_ptr() : nullptr, residual.defined() ? residual.data_ptr() : nullptr, l.rows,
+                              l.dim, l.out, row_stride(x), row_stride(weight), l.out, residual.defined() ? row_stride(residual) : 0,
+                              padded, dtype_id(x.scalar_type()), bias.defined() ? dtype_id(bias.scalar_type()) : FPT_FP32,
+                              int(function), int(degree), int(source), const_cast<uint32_t*>(status_word()), stream_of(x));
+    TORCH_CHECK(rc != FPT_ERR_UNKNOWN_PROGRAM, "Unsupported activation degree: ", degree);
+    check_status(rc, "fpt_linear");
+    return {out, slope};
+}
+
+Tensor linear_act(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int64_t function,
+                  int64_t degree, int64_t source) {
+    return std::get<0>(run_linear(x, weight, bias, residual, function, degree, source, false));
+}
+
+std::tuple<Tensor, Tensor> linear_act_slope(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
+                                            int64_t function, int64_t degree, int64_t source) {
+    return run_linear(x, weight, bias, residual, function, degree, source, true);
+}
+
+// dx, dW, db; empty where not wanted.  slope: empty for no activation.  bias_dtype: 0 float16, 1 bfloat16, 2 float32.
+std::tuple<Tensor, Tensor, Tensor> linear_act_bwd(const Tensor& dy_in, const Tensor& slope, const OptTensor& x_in, const OptTensor& weight_in,
+                                                  at::IntArrayRef x_shape, int64_t out, int64_t bias_dtype, bool want_x, bool want_weight,
+                                                  bool want_bias) {
+    TORCH_CHECK(dy_in.is_cuda(), "the gradient must be a CUDA tensor");
+    TORCH_CHECK(dy_in.scalar_type() == at::kHalf || dy_in.scalar_type() == at::kBFloat16, "the gradient must be float16 or bfloat16");
+    TORCH_CHECK(!x_shape.empty() && out > 0 && dy_in.dim() == int64_t(x_shape.size()) && dy_in.size(-1) == out, "the gradient must have the shape of the result");
+    TORCH_CHECK((!want_x || weight_in) && (!want_weight || x_in), "the weight and x are needed for each other's gradient");
+    TORCH_CHECK(bias_dtype >= FPT_FP16 && bias_dtype <= FPT_FP32, "unknown bias dtype");
+    const int64_t dim = x_shape.back(), rows = dy_in.numel() / out, padded = (out + 7) / 8 * 8;
+    int64_t expected = 1;
+    for (size_t i = 0; i + 1 < x_shape.size(); ++i) expected *= x_shape[i];
+    TORCH_CHECK(rows == expected, "the gradient must have the shape of the result");
+    TORCH_CHECK(slope.numel() == 0 || (slope.scalar_type() == at::kHalf && slope.is_contiguous() && slope.numel() == rows * padded &&
+                                       slope.device() == dy_in.device()), "the slope does not fit the gradient");
+    for (const OptTensor* t : {&x_in, &weight_in})
+        if (t->has_value())
+            TORCH_CHECK((*t)->scalar_type() == dy_in.scalar_type() && (*t)->device() == dy_in.device(), "x and weight must have the gradient's dtype and device");
+    TORCH_CHECK(!want_x || (weight_in->dim() == 2 && weight_in->size(0) == out && weight_in->size(1) == dim), "the weight does not fit the gradient");
+    TORCH_CHECK(!want_weight || x_in->sizes() == x_shape, "x does not fit the gradient");
+    poll_linear_status();
+    const c10::cuda::CUDAGuard guard(dy_in.device());
+    const int dtype = dtype_id(dy_in.scalar_type());
+    Tensor dx = at::empty(want_x ? x_shape : at::IntArrayRef({0}), dy_in.options(), at::MemoryFormat::Contiguous);
+    Tensor dw = at::empty({want_weight ? out : 0, dim}, dy_in.options(), at::MemoryFormat::Contiguous);
+    Tensor db = at::empty({want_bias ? out : 0}, dy_in.options().dtype(bias_dtype == FPT_FP32 ? at::kFloat : bias_dtype == FPT_BF16 ? at::kBFloat16 : at::kHalf));
+    const Tensor dy = rows ? as_rows(dy_in, rows, out) : dy_in.reshape({0, out});
+    const bool products = want_x || want_weight;
+    Tensor dz = dy;
+    const bool copy = rows && products && (slope.numel() || !loadable(dy));
+    if (copy) dz = at::empty({rows, padded}, dy.options(), at::MemoryFormat::Contiguous);
+    if (copy || want_bias) {
+        const int64_t bytes = want_bias ? fpt_linear_grad_act_workspace_bytes(rows, out) : 0;
+        Tensor workspace = at::empty({bytes}, dy.options().dtype(at::kByte));
+        check_status(fpt_linear_grad_act(copy ? dz.data_ptr() : nullptr, want_bias ? db.data_ptr() : nullptr, dy.data_ptr(),
+                                         slope.numel() ? slope.data_ptr() : nullptr, bytes ? workspace.data_ptr() : nullptr, bytes, rows, out,
+                                         padded, rows ? row_stride(dy) : out, padded, dtype, int(bias_dtype), stream_of(dy)),
+                     "fpt_linear_grad_act");
+    }
+    void* status = const_cast<uint32_t*>(status_word());
+    const int64_t dz_ld = copy ? padded : rows ? row_stride(dz) : padded;
+    if (want_x && rows) {
+        const Tensor weight = as_operand(*weight_in, out, dim);
+        check_status(fpt_linear_grad_input(dx.data_ptr(), dz.data_ptr(), weight.data_ptr(), rows, dim, out, dim, dz_ld, row_stride(weight), dtype,
+                                           status, stream_of(dy)),
+                     "fpt_linear_grad_input");
+    }
+    if (want_weight) {
+        const Tensor x = rows ? as_operand(*x_in, rows, dim) : *x_in;
+        check_status(fpt_linear_grad_weight(dw.data_ptr(), dz.data_ptr(), x.data_ptr(), rows, dim, out, dim, dz_ld, rows ? row_stride(x) : dim, dtype,
+                                            status, stream_of(dy)),
+                     "fpt_linear_grad_weight");
+    }
+    return {dx, dw, db};
+}
+
+Tensor call_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int64_t function,
+                   int64_t degree, int64_t source) {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::linear_act", "").typed<decltype(linear_act)>();
+    return op.call(x, weight, bias, residual, function, degree, source);
+}
+
+struct LinearFunction : torch::autograd::Function<LinearFunction> {
+    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias,
+                          const OptTensor& residual, int64_t function, int64_t degree, int64_t source) {
+        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::linear_act_slope", "").typed<decltype(linear_act_slope)>();
+        at::AutoDispatchBelowADInplaceOrView below;
+        const bool want_x = x.requires_grad(), want_w = weight.requires_grad(), want_b = bias && bias->requires_grad();
+        Tensor out, slope;
+        if (function == FPT_FN_NONE || !(want_x || want_w || want_b)) {          // the slope is 1, or nobody asks for it
+            out = call_linear(x, weight, bias, residual, function, degree, source);
+            slope = at::empty({0, (weight.size(0) + 7) / 8 * 8}, x.options().dtype(at::kHalf));
+        } else {
+            std::tie(out, slope) = op.call(x, weight, bias, residual, function, degree, source);
+        }
+        ctx->save_for_backward({want_w ? x : Tensor(), want_x ? weight : Tensor(), slope});
+        ctx->saved_data["shape"] = x.sizes().vec();
+        ctx->saved_data["out"] = weight.size(0);
+        ctx->saved_data["bias_dtype"] = int64_t(bias ? dtype_id(bias->scalar_type()) : FPT_FP32);
+        ctx->saved_data["x"] = want_x;
+        ctx->saved_data["weight"] = want_w;
+        ctx->saved_data["bias"] = want_b;
+        ctx->saved_data["residual"] = residual && residual->requires_grad();
+        return out;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        no_second_gradient("linear_act");
+        const auto saved = ctx->get_saved_variables();
+        const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+        const bool want_x = ctx->saved_data["x"].toBool(), want_w = ctx->saved_data["weight"].toBool(), want_b = ctx->saved_data["bias"].toBool();
+        torch::autograd::variable_list out(7);
+        if (want_x || want_w || want_b) {
+            static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::linear_act_bwd", "").typed<decltype(linear_act_bwd)>();
+            auto d = op.call(grads[0], saved[2], opt(saved[0]), opt(saved[1]), ctx->saved_data["shape"].toIntVector(), ctx->saved_data["out"].toInt(),
+                             ctx->saved_data["bias_dtype"].toInt(), want_x, want_w, want_b);
+            if (want_x) out[0] = std::get<0>(d);
+            if (want_w) out[1] = std::get<1>(d);
+            if (want_b) out[2] = std::get<2>(d);
+        }
+        if (ctx->saved_data["residual"].toBool()) out[3] = grads[0];
+        return out;
+    }
+};
+
+Tensor linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int64_t function,
+                       int64_t degree, int64_t source) {
+    const bool wanted = at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()) ||
+                                                       (residual && residual->requires_grad()));
+    if (!wanted) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        return call_linear(x, weight, bias, residual, function, degree, source);
+    }
+    return LinearFunction::apply(x, weight, bias, residual, function, degree, source);
+}
+
+// the eager doors: off the GPU the checks run here, where no kernel would be found
+Tensor enter_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int64_t function,
+                    int64_t degree, int64_t source) {
+    if (!x.is_cuda()) check_linear(x, weight, bias, residual, function, degree, source);
+    return call_linear(x, weight, bias, residual, function, degree, source);
+}
+
 std::tuple<Tensor, Tensor> enter_qk_rope(const Tensor& q, const Tensor& k, const OptTensor& q_weight, const OptTensor& k_weight,
                                          const Tensor& increments, const OptTensor& positions, const std::vector<int64_t>& sections,
                                          int64_t order, int64_t pairing, bool norm, double eps) {
@@ -271,17 +503,27 @@ TORCH_LIBRARY_FRAGMENT(fpt_b200, m) {
     m.def("qk_norm_rope_bwd(Tensor dq_out, Tensor dk_out, Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, "
           "Tensor phase_increments, Tensor? positions, int[] sections, int section_order, int pairing, float eps, "
           "bool want_q_weight, bool want_k_weight) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("linear_act(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int function, int degree, int source) -> Tensor");
+    m.def("linear_act_slope(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int function, int degree, int source) -> (Tensor, Tensor)");
+    m.def("linear_act_bwd(Tensor dy, Tensor slope, Tensor? x, Tensor? weight, int[] x_shape, int out, int bias_dtype, bool want_x, "
+          "bool want_weight, bool want_bias) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(fpt_b200, CUDA, m) {
     m.impl("qk_rope", &qk_rope);
     m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd);
+    m.impl("linear_act", &linear_act);
+    m.impl("linear_act_slope", &linear_act_slope);
+    m.impl("linear_act_bwd", &linear_act_bwd);
 }
 
 TORCH_LIBRARY_IMPL(fpt_b200, Autograd, m) {
     m.impl("qk_rope", &qk_rope_autograd);
+    m.impl("linear_act", &linear_autograd);
 }
 
 void register_block_operators(pybind11::module_& m) {
     m.def("qk_rope", &enter_qk_rope);
+    m.def("linear_act", &enter_linear);
+    m.def("poll_linear_status", &poll_linear_status);
 }

@@ -47,6 +47,7 @@ enum { FPT_FP16 = 0, FPT_BF16 = 1 };
 enum { FPT_FP32 = 2 }; /* fpt_qk_rope and its backward pass, and weights and biases where a comment says so */
 enum { FPT_SRC_CURRENT = 0, FPT_SRC_SOLLYA = 1 };
 enum { FPT_FN_SIGMOID = 0, FPT_FN_TANH = 1, FPT_FN_SWISH = 2, FPT_FN_ERF = 3, FPT_FN_GELU = 4 };
+enum { FPT_FN_NONE = -1 }; /* fpt_linear: no activation */
 enum { FPT_FWD = 0, FPT_BWD = 1 };
 /* degree: 3..6 selects the polynomial of that degree; 0 selects the native special-function-unit
  * (MUFU) control that shares the same memory code. */
@@ -394,6 +395,38 @@ int fpt_qk_norm_rope_bwd(void* dq, void* dk, void* dq_weight, void* dk_weight, c
                          const int64_t* dq_out_strides, const int64_t* dk_out_strides, int pairing, float eps, int dtype,
                          int weight_dtype, fpt_stream_t stream);
 
+/* ---- a linear layer with its bias, its activation and the residual connection in the epilogue
+ *          y = act(x W^T + b) + r
+ *      (no counterpart in the reference, which multiplies with the library and applies fpt_unary to the stored product).
+ *      x [rows, dim], weight [out_features, dim] (rows contiguous, 16-byte aligned, strides *_ld in elements, multiples of
+ *      8; dim a multiple of 8), out [rows, out_features], residual as out or null: dtype FPT_FP16 or FPT_BF16; bias
+ *      [out_features] of bias_dtype (FPT_FP32 too) or null.  out, residual and slope rows of any alignment (16 bytes are
+ *      faster); out must not overlap any input.
+ *      function: FPT_FN_NONE, FPT_FN_SIGMOID, FPT_FN_TANH, FPT_FN_SWISH or FPT_FN_GELU.  degree 0: the function itself in
+ *      fp32 on the fp32 sums, one rounding at the end.  degree 3..6: the packed polynomial program of fpt_unary on the sums
+ *      rounded to dtype (with a residual: its value plus the residual, rounded again).
+ *      slope (fp16 [rows, out_features], whatever dtype) or null: act'(x W^T + b) for fpt_linear_grad_act; with a degree
+ *      the derivative program of the same degree.
+ *      status: one word the device can write and the host can read (mapped host memory serves; null: not reported): a
+ *      bounded device-side wait that runs out stores 0x80000000 | where there, and the outputs of that call are invalid.
+ *      It is not read when a call starts. */
+int fpt_linear(void* out, void* slope, const void* x, const void* weight, const void* bias, const void* residual,
+               int64_t rows, int64_t dim, int64_t out_features, int64_t x_ld, int64_t w_ld, int64_t out_ld,
+               int64_t residual_ld, int64_t slope_ld, int dtype, int bias_dtype, int function, int degree, int source,
+               void* status, fpt_stream_t stream);
+/* Its gradient in three parts.  dz = dy * slope (slope null: dz = dy) rounded to dtype, dbias = its column sums before that
+ *      rounding, in a fixed order; dz or dbias null where not wanted.  dz and slope rows are 16-byte aligned and padded to
+ *      a multiple of 8 columns (the padding of dz is written with zeros); workspace (4-byte aligned) for dbias. */
+int64_t fpt_linear_grad_act_workspace_bytes(int64_t rows, int64_t out_features);
+int fpt_linear_grad_act(void* dz, void* dbias, const void* dy, const void* slope, void* workspace, int64_t workspace_bytes,
+                        int64_t rows, int64_t out_features, int64_t dz_ld, int64_t dy_ld, int64_t slope_ld, int dtype,
+                        int bias_dtype, fpt_stream_t stream);
+/*      dx [rows, dim] = dz W,   dW [out_features, dim] = dz^T x (zeros without rows); alignment of the operands as above. */
+int fpt_linear_grad_input(void* dx, const void* dz, const void* weight, int64_t rows, int64_t dim, int64_t out_features,
+                          int64_t dx_ld, int64_t dz_ld, int64_t w_ld, int dtype, void* status, fpt_stream_t stream);
+int fpt_linear_grad_weight(void* dw, const void* dz, const void* x, int64_t rows, int64_t dim, int64_t out_features,
+                           int64_t dw_ld, int64_t dz_ld, int64_t x_ld, int dtype, void* status, fpt_stream_t stream);
+
 /* ---- diagnostic: one 128x128x128 bf16 tile through the tensor-core building blocks of the attention kernel
  *      (no counterpart in the reference).  a, b: bf16 [128,128] row-major; c: fp32 [128,128];
  *      mode 0: c = a * b^T (both operands K-major in shared memory); mode 1: c = a * b (a staged in tensor memory,
@@ -433,6 +466,9 @@ int fpt_selftest_bounded_wait(void* status, void* report, int64_t limit_ns, int 
  * "gate_up_tile_rows" names a height;
  * key "gate_up_pair_wide": 1 gives a pair two hidden tiles per row tile (a 256 x 256 output tile) where the number of hidden
  * tiles is even, 0 (default) one: measured slower (no accumulator left to alternate);
+ * key "linear_tokens": fpt_linear and its products: 16, 32, 64 or 128 tokens per tile of the few-row form, 0 the form on
+ * pairs of CTAs, -1 (default) by size; key "linear_split": blocks that share an output tile of the few-row form along K
+ * (1..8), 0 (default) by size;
  * key "gate_up_tile_rows": rows per tile of the single-CTA forms, 128 or 256; 0 (default) = 256 for one group (both halves
  * of a tile share every weight tile: fewer bytes per product, which under the power cap is the faster form), 128 for
  * grouped problems (a ragged group wastes less of a smaller tile). */
