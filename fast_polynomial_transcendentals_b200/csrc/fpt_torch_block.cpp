@@ -139,7 +139,15 @@ Rope check_rope(const Tensor& q, const Tensor& k, const OptTensor& q_weight, con
     return r;
 }
 
-Tensor rows_contiguous(const Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
+// What the kernels take as it is: heads contiguous and on 16-byte boundaries, no more than 2 GB from a token's first to its
+// last; anything else is copied.
+Tensor rows_contiguous(const Tensor& t) {
+    const int64_t item = t.element_size();
+    bool fits = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    for (int d = 0; d < 3; ++d) fits = fits && (t.size(d) < 2 || t.stride(d) * item % 16 == 0);
+    fits = fits && (t.size(2) < 2 || t.stride(2) <= 0x7fffffff / item / t.size(2));
+    return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
 
 const void* pointer(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
 

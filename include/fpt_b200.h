@@ -365,7 +365,7 @@ int fpt_attention_bwd_routed(void* dq, void* dk, void* dv, const void* dout, con
  *      fpt_rope_apply, rotates by 0 .. seq - 1 in fp16 arithmetic and has no gradient).
  *          u = x / sqrt(mean(x^2) + eps),   y = R (weight * u)
  *      q, k: [batch, seq, heads, head_dim] by their three outer strides in elements (batch, seq, head; head_dim
- *      contiguous; any alignment, 16-byte rows are faster); q_out, k_out: contiguous, 16-byte aligned, of the same shape;
+ *      contiguous, every head on a 16-byte boundary); q_out, k_out: contiguous, 16-byte aligned, of the same shape;
  *      either side may have no heads.  dtype FPT_FP16, FPT_BF16 or FPT_FP32; weights [head_dim] of weight_dtype, or null
  *      for ones.  Arithmetic is fp32, rounded once.
  *      head_dim: a multiple of 8 up to 256.  pairs: a multiple of 4, 2 pairs <= head_dim; dimensions from 2 pairs on pass
