@@ -34,6 +34,7 @@ int tuning_attention_cta_pair();    // attention forward on pairs of CTAs (cta_g
 int tuning_gate_up_tile_rows();     // gate / up projection: rows per tile, 128 or 256 (0: 256 for dense, 128 for grouped problems)
 int tuning_rope_heads_per_block();   // fused RoPE: heads one block rotates (0: all of them)
 int tuning_linear_tokens();      // linear layer: tokens per tile of the few-row form (16, 32, 64, 128), 0 the pair form, -1 (default) by size
+int tuning_linear_columns();     // linear layer, pair form: columns of an output tile (64 .. 256, a multiple of 32), 0 (default) by size
 int tuning_linear_split();       // linear layer, few-row form: blocks that share an output tile along K, 0 (default) by size
 int tuning_attention_split();    // attention forward, column-split score-mod warps: 0 never, 1 soft-capped mode (default), 2 sigmoid mode too
 

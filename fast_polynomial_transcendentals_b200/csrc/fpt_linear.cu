@@ -10,7 +10,7 @@
 // TMA into 128-byte-swizzled tiles: K-major tiles of [rows x 64 k], or MN-major ones of two panels [64 k x 64 rows], so
 // that no operand is ever transposed in memory.  Two forms:
 //
-//   linear_pair_kernel    many rows.  Persistent pairs of CTAs (cta_group::2), 256 x 256 output tiles, two accumulators in
+//   linear_pair_kernel    many rows.  Persistent pairs of CTAs (cta_group::2), output tiles of 256 rows x 64 .. 256 columns, two accumulators in
 //                         turn so that the epilogue of one tile runs under the products of the next; bound by the tensor
 //                         pipe (and, in long runs, by the power cap).
 //   linear_split_kernel   few rows.  The weight is the 128-row operand and the tokens are the columns (16 .. 128 of them): a
@@ -43,6 +43,7 @@ using namespace sm100;
 constexpr int kBlockK = 64;
 constexpr uint32_t kTileBytes = 128 * 128;          // 128 rows x 64 values
 constexpr uint32_t kPanelBytes = kTileBytes / 2;    // MN-major: 64 k x 64 rows
+constexpr int kMaxRing = 12;                        // stages of a ring
 constexpr int kBandTiles = 16;                      // 256-row tiles per band: 4096 rows, see fpt_gate_up_swiglu.cu
 
 enum : uint32_t { kWaitEmpty = 0x51, kWaitFull, kWaitAccEmpty, kWaitAccFull };
@@ -63,13 +64,21 @@ struct LinearParams {
     int m, n, k_blocks;
     int m_tiles, n_tiles;
     int split;                      // blocks per cluster (split form)
+    int columns;                    // columns of an output tile (pair form), a multiple of 32
+    int ring;                       // stages of the ring and their size (pair form)
+    uint32_t stage_bytes;
     int bias_dtype;
     bool vec_out, vec_res, vec_slope, vec_bias;
+    bool staged;                    // out, residual and slope rows all start on 16-byte boundaries (pair form)
     Activation act;
     uint32_t* status;
 };
 
 // ---- waits --------------------------------------------------------------------------------------------------------
+
+// Launched while the kernel before it drains (launch_early below): barriers and tensor memory are set up by then, and nothing of
+// global memory is touched before this.
+__device__ __forceinline__ void wait_for_inputs() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __noinline__ void report(uint32_t* status, uint32_t where) {
     volatile uint32_t* s = status;
@@ -251,6 +260,103 @@ __device__ __forceinline__ void finish(const LinearParams& p, float (&z)[N], int
     }
 }
 
+// ---- the same for a warp that holds 32 rows x 32 columns, a row per lane -------------------------------------------------
+//
+// A lane's row is 64 contiguous bytes; read or written from registers, a warp's accesses would touch 32 lines with 16 bytes
+// each.  The chunk goes through 2 KB of shared memory instead, four lanes to a row: eight rows of 64 bytes per access.  The
+// 16-byte piece q of row r lies at piece q ^ (r / 2 % 4): no bank conflicts on either side.
+
+struct Stage {
+    alignas(16) uint4 piece[32 * 4];
+};
+__device__ __forceinline__ int stage_at(int row, int piece) { return row * 4 + (piece ^ ((row >> 1) & 3)); }
+
+// rows `row0 + 8 i + lane / 4`, i = 0 .. 3; `valid` rows exist
+__device__ __forceinline__ void load_rows(uint4 (&v)[4], const uint16_t* base, int64_t ld, int lane, int valid) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + (lane >> 2);
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (r < valid) v[i] = *reinterpret_cast<const uint4*>(base + int64_t(r) * ld + 8 * (lane & 3));
+    }
+}
+__device__ __forceinline__ void rows_to_stage(Stage& s, const uint4 (&v)[4], int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s.piece[stage_at(8 * i + (lane >> 2), lane & 3)] = v[i];
+}
+__device__ __forceinline__ void stage_to_rows(const Stage& s, uint16_t* base, int64_t ld, int lane, int valid) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + (lane >> 2);
+        const uint4 v = s.piece[stage_at(r, lane & 3)];
+        if (r < valid) *reinterpret_cast<uint4*>(base + int64_t(r) * ld + 8 * (lane & 3)) = v;
+    }
+}
+
+// All 32 lanes, converged.  `res`: this chunk of the residual as load_rows left it (where p.residual).
+template <int DT>
+__device__ __forceinline__ void finish_staged(const LinearParams& p, float (&z)[32], const uint4 (&res)[4], Stage& s, int row0, int column, int lane) {
+    const int valid = p.m - row0;
+    if (p.bias) {
+        if (p.bias_dtype != FPT_FP32 && p.vec_bias) {
+            const uint4* b = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.bias) + column);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const uint4 q = b[v];
+                const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool bf = p.bias_dtype == FPT_BF16;
+                    z[8 * v + 2 * i] += bf ? Sfu<kBf16>::lo(words[i]) : Sfu<kFp16>::lo(words[i]);
+                    z[8 * v + 2 * i + 1] += bf ? Sfu<kBf16>::hi(words[i]) : Sfu<kFp16>::hi(words[i]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) z[i] += load_any(p.bias, p.bias_dtype, column + i);
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {                   // halves: fewer registers
+        float (&half)[16] = *reinterpret_cast<float (*)[16]>(z + 16 * h);
+        float d[16];
+        activate<DT, 16>(p.act, half, d, p.slope != nullptr);
+        if (p.slope) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+                s.piece[stage_at(lane, 2 * h + q)] = make_uint4(Sfu<kFp16>::pack(d[8 * q], d[8 * q + 1]), Sfu<kFp16>::pack(d[8 * q + 2], d[8 * q + 3]),
+                                                                Sfu<kFp16>::pack(d[8 * q + 4], d[8 * q + 5]), Sfu<kFp16>::pack(d[8 * q + 6], d[8 * q + 7]));
+        }
+    }
+    if (p.slope) {
+        __syncwarp();
+        stage_to_rows(s, p.slope + int64_t(row0) * p.slope_ld + column, p.slope_ld, lane, valid);
+        __syncwarp();
+    }
+    if (p.residual) {
+        rows_to_stage(s, res, lane);
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint4 v = s.piece[stage_at(lane, q)];
+            const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                z[8 * q + 2 * i] += Sfu<DT>::lo(words[i]);
+                z[8 * q + 2 * i + 1] += Sfu<DT>::hi(words[i]);
+            }
+        }
+        // each lane overwrites its own row next: nobody else reads it before the barrier below
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        s.piece[stage_at(lane, q)] = make_uint4(Sfu<DT>::pack(z[8 * q], z[8 * q + 1]), Sfu<DT>::pack(z[8 * q + 2], z[8 * q + 3]),
+                                                Sfu<DT>::pack(z[8 * q + 4], z[8 * q + 5]), Sfu<DT>::pack(z[8 * q + 6], z[8 * q + 7]));
+    __syncwarp();
+    stage_to_rows(s, static_cast<uint16_t*>(p.out) + int64_t(row0) * p.out_ld + column, p.out_ld, lane, valid);
+    __syncwarp();
+}
+
 // kind::f16 instruction descriptor with both operands of this data type (umma_idesc_bf16 is the bf16 one)
 template <int DT>
 __host__ __device__ constexpr uint32_t instruction(uint32_t m, uint32_t n, bool a_mn, bool b_mn) {
@@ -264,15 +370,15 @@ constexpr uint32_t kStep16 = MN ? 2048u / 16u : 2u;
 
 // ---- many rows: pairs of CTAs ---------------------------------------------------------------------------------------
 
-constexpr int kPairRing = 6;
+constexpr uint32_t kRingBytes = 192 * 1024;
 constexpr int kPairThreads = 384;       // TMA, product and allocation warps, one idle, eight epilogue warps
 
 struct PairSmem {
-    alignas(1024) uint8_t a[kPairRing][kTileBytes];
-    alignas(1024) uint8_t b[kPairRing][kTileBytes];
-    alignas(8) uint64_t full[kPairRing];
-    uint64_t empty[kPairRing];
+    alignas(1024) uint8_t ring[kRingBytes];        // stages of an A tile and a B tile, as many as fit
+    alignas(8) uint64_t full[kMaxRing];
+    uint64_t empty[kMaxRing];
     uint64_t acc_full[2], acc_empty[2];
+    Stage stage[8];
     uint32_t tmem_base;
     uint32_t abort_flag;
 };
@@ -287,21 +393,22 @@ __device__ __forceinline__ PairTile pair_tile(const LinearParams& p, int tile) {
     const int band = tile / per_band, r = tile - band * per_band;
     const int in_band = min(kBandTiles, p.m_tiles - band * kBandTiles);
     const int column = r / in_band;
-    return PairTile{(band * kBandTiles + r - column * in_band) * 256, column * 256};
+    return PairTile{(band * kBandTiles + r - column * in_band) * 256, column * p.columns};
 }
 
 template <bool MN>
-__device__ __forceinline__ void load_pair(uint8_t* tile, const CUtensorMap* map, uint32_t bar, int kb, int row) {
+__device__ __forceinline__ void load_pair(uint8_t* tile, const CUtensorMap* map, uint32_t bar, int kb, int row, bool both) {
     if constexpr (MN) {
         tma_load_4d_pair(tile, map, bar, row, kb * kBlockK, 0, 0);
-        tma_load_4d_pair(tile + kPanelBytes, map, bar, row + 64, kb * kBlockK, 0, 0);
+        if (both) tma_load_4d_pair(tile + kPanelBytes, map, bar, row + 64, kb * kBlockK, 0, 0);
     } else {
         tma_load_4d_pair(tile, map, bar, kb * kBlockK, row, 0, 0);
     }
 }
 
-// Each CTA of the pair holds 128 rows of A and of B and receives 128 rows x 256 columns of D; the hand-overs are those of
-// gate_up_swiglu_pair_kernel.
+// Each CTA of the pair holds 128 rows of A and half the tile's columns' rows of B and receives 128 rows x p.columns columns of
+// D; the hand-overs are those of gate_up_swiglu_pair_kernel.  The host picks the number of columns so that the tiles come
+// out even over the pairs.
 template <int DT, bool A_MN, bool B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ LinearParams p) {
@@ -311,7 +418,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     const uint32_t rank = cluster_cta_rank();
     volatile uint32_t* abort_flag = &sm.abort_flag;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kPairRing; ++s) {
+        for (int s = 0; s < p.ring; ++s) {
             mbar_init(&sm.full[s], 1);
             mbar_init(&sm.empty[s], 1);
         }
@@ -332,31 +439,36 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     cluster_sync_all();
     tc_fence_after_sync();
     const uint32_t tmem = sm.tmem_base;
+    wait_for_inputs();
     const int tiles = p.m_tiles * p.n_tiles;
     const int first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
 
     if (warp == 0) {
         if (lane == 0) {
-            uint32_t it = 0;
+            uint32_t s = 0, turn = 0;                       // stage, and how often the ring has gone round
             bool ok = true;
+            const int b_rows = p.columns / 2;
+            const uint32_t bytes = 2 * (kTileBytes + (B_MN ? (b_rows > 64 ? 2u : 1u) * kPanelBytes : uint32_t(b_rows) * 128u));
             for (int tile = first_tile; tile < tiles && ok; tile += tile_step) {
                 const PairTile t = pair_tile(p, tile);
-                for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
-                    const uint32_t s = it % kPairRing, use = it / kPairRing;
-                    if (use > 0) ok = wait(&sm.empty[s], (use - 1u) & 1u, abort_flag, p.status, kWaitEmpty);
+                for (int kb = 0; kb < p.k_blocks; ++kb) {
+                    if (turn > 0) ok = wait(&sm.empty[s], (turn - 1u) & 1u, abort_flag, p.status, kWaitEmpty);
                     if (!ok) break;
                     const uint32_t bar = map_to_cta(smem_u32(&sm.full[s]), 0);
-                    if (rank == 0) mbar_arrive_expect_tx(&sm.full[s], 4 * kTileBytes);
-                    load_pair<A_MN>(sm.a[s], &map_a, bar, kb, t.row0 + int(rank) * 128);
-                    load_pair<B_MN>(sm.b[s], &map_b, bar, kb, t.column0 + int(rank) * 128);
+                    uint8_t* stage = sm.ring + s * p.stage_bytes;
+                    if (rank == 0) mbar_arrive_expect_tx(&sm.full[s], bytes);
+                    load_pair<A_MN>(stage, &map_a, bar, kb, t.row0 + int(rank) * 128, true);
+                    load_pair<B_MN>(stage + kTileBytes, &map_b, bar, kb, t.column0 + int(rank) * b_rows, b_rows > 64);
+                    if (++s == uint32_t(p.ring)) s = 0, ++turn;
                 }
             }
         }
     } else if (warp == 1 && rank == 0) {
         const bool elected = elect_one();
-        constexpr uint32_t idesc = instruction<DT>(256, 256, A_MN, B_MN);
+        const uint32_t idesc = instruction<DT>(256, uint32_t(p.columns), A_MN, B_MN);
         constexpr uint32_t desc_hi = umma_smem_desc_hi(1024);
-        uint32_t it = 0, local = 0;
+        const uint32_t a_first = tile_lo<A_MN>(sm.ring), b_first = tile_lo<B_MN>(sm.ring + kTileBytes);
+        uint32_t s = 0, turn = 0, local = 0;
         bool ok = true;
         for (int tile = first_tile; tile < tiles && ok; tile += tile_step, ++local) {
             const uint32_t a = local & 1u, use = local >> 1;
@@ -368,46 +480,59 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 }
                 tc_fence_after_sync();
             }
-            for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
-                const uint32_t s = it % kPairRing;
-                ok = wait(&sm.full[s], (it / kPairRing) & 1u, abort_flag, p.status, kWaitFull);
+            for (int kb = 0; kb < p.k_blocks; ++kb) {
+                ok = wait(&sm.full[s], turn & 1u, abort_flag, p.status, kWaitFull);
                 if (!ok) break;
                 tc_fence_after_sync();
-                const uint32_t a_lo = tile_lo<A_MN>(sm.a[s]), b_lo = tile_lo<B_MN>(sm.b[s]);
+                const uint32_t a_lo = a_first + s * (p.stage_bytes / 16u), b_lo = b_first + s * (p.stage_bytes / 16u);
 #pragma unroll
                 for (uint32_t k = 0; k < kBlockK / 16; ++k)
                     if (elected) umma_ss_words_pair(tmem + a * 256u, a_lo + k * kStep16<A_MN>, b_lo + k * kStep16<B_MN>, desc_hi, idesc, (kb > 0 || k > 0) ? 1u : 0u);
                 if (elected) umma_commit_pair(&sm.empty[s], 3);
+                if (++s == uint32_t(p.ring)) s = 0, ++turn;
             }
             if (ok && elected) umma_commit_pair(&sm.acc_full[a], 3);
         }
     } else if (warp >= 4) {
-        // four warps hold the 128 rows (a warp reads the 32 lanes of its number modulo 4); two such sets take 128 columns each
+        // four warps hold the 128 rows (a warp reads the 32 lanes of its number modulo 4); two such sets take the 32-column
+        // chunks in turn
         const uint32_t lane_base = uint32_t(32 * (warp & 3)) << 16;
-        const int half = (warp - 4) >> 2;
+        const int set = (warp - 4) >> 2;
+        Stage& stage = sm.stage[warp - 4];
         uint32_t local = 0;
         bool ok = true;
         for (int tile = first_tile; tile < tiles && ok; tile += tile_step, ++local) {
             const PairTile t = pair_tile(p, tile);
             const uint32_t a = local & 1u;
+            const int row0 = t.row0 + int(rank) * 128 + 32 * (warp & 3), valid = p.m - row0;
+            const int column_end = min(p.n, t.column0 + p.columns);
+            uint4 res[4];
+            const auto prefetch = [&](int column) {                     // the residual of a chunk, ahead of its turn
+                if (p.residual && p.staged && column + 32 <= column_end && valid > 0)
+                    load_rows(res, static_cast<const uint16_t*>(p.residual) + int64_t(row0) * p.res_ld + column, p.res_ld, lane, valid);
+            };
+            prefetch(t.column0 + set * 32);
             ok = wait(&sm.acc_full[a], (local >> 1) & 1u, abort_flag, p.status, kWaitAccFull);
             if (!ok) break;
             tc_fence_after_sync();
-            const int row = t.row0 + int(rank) * 128 + 32 * (warp & 3) + lane;
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-                const int column = t.column0 + half * 128 + c * 32;
-                if (column >= p.n) break;
+            for (int c = set * 32; c < p.columns; c += 64) {
+                const int column = t.column0 + c;
+                if (column >= p.n || valid <= 0) break;
                 uint32_t acc[32];
-                tmem_ld_32x32b_x32(tmem + lane_base + a * 256u + uint32_t(half * 128 + c * 32), acc);
+                tmem_ld_32x32b_x32(tmem + lane_base + a * 256u + uint32_t(c), acc);
                 tmem_ld_wait();
-                if (row < p.m) {
-                    float z[32];
+                float z[32];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) z[i] = __uint_as_float(acc[i]);
-                    finish<DT, 32>(p, z, row, column);
+                for (int i = 0; i < 32; ++i) z[i] = __uint_as_float(acc[i]);
+                if (p.staged && column + 32 <= p.n) {
+                    uint4 mine[4] = {res[0], res[1], res[2], res[3]};
+                    prefetch(column + 64);
+                    finish_staged<DT>(p, z, mine, stage, row0, column, lane);
+                } else {
+                    if (lane < valid) finish<DT, 32>(p, z, row0 + lane, column);
+                    __syncwarp();
                 }
-                __syncwarp();
             }
             tc_fence_before_sync();
             __syncwarp();
@@ -429,24 +554,16 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 constexpr int kSplitThreads = 256;
 constexpr int kMaxSplit = 8;
 
-template <int TOKENS>
+// Barriers, then (1024-byte aligned) the ring of weight and token tiles, as many stages as the launch has memory for; after
+// the last product its first 512 TOKENS bytes hold this block's sums, [token][output].
 struct SplitSmem {
-    static constexpr uint32_t kXBytes = TOKENS * 128;
-    static constexpr int kRing = 108 * 1024 / int(kTileBytes + kXBytes);       // two blocks an SM
-    struct Ring {
-        alignas(1024) uint8_t w[kRing][kTileBytes];
-        alignas(1024) uint8_t x[kRing][kXBytes];
-    };
-    union {
-        Ring ring;
-        float partial[TOKENS][128];               // after the last product: this block's sums, [token][output]
-    };
-    alignas(8) uint64_t full[kRing];
-    uint64_t empty[kRing];
+    uint64_t full[kMaxRing], empty[kMaxRing];
     uint64_t acc_full;
     uint32_t tmem_base;
     uint32_t abort_flag;
 };
+constexpr uint32_t kSplitRingOffset = 1024;
+static_assert(sizeof(SplitSmem) <= kSplitRingOffset, "barriers before the ring");
 
 __device__ __forceinline__ float4 load_cluster(uint32_t address) {
     float4 v;
@@ -459,11 +576,13 @@ __device__ __forceinline__ float4 load_cluster(uint32_t address) {
 template <int DT, int TOKENS, bool W_MN>
 __global__ void __launch_bounds__(kSplitThreads, 2)
 linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ LinearParams p) {
-    using Smem = SplitSmem<TOKENS>;
-    constexpr int kRing = Smem::kRing;
+    constexpr uint32_t kXBytes = TOKENS * 128, kStageBytes = kTileBytes + kXBytes;
     constexpr uint32_t kColumns = TOKENS < 32 ? 32 : TOKENS;
     extern __shared__ uint8_t smem_raw[];
-    Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    SplitSmem& sm = *reinterpret_cast<SplitSmem*>(base);
+    uint8_t* ring = base + kSplitRingOffset;
+    float (*partial)[128] = reinterpret_cast<float (*)[128]>(ring);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = p.split > 1 ? int(cluster_cta_rank()) : 0;
     volatile uint32_t* abort_flag = &sm.abort_flag;
@@ -471,7 +590,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     const int output0 = tile / p.m_tiles * 128, token0 = tile % p.m_tiles * TOKENS;
     const int kb0 = int(int64_t(p.k_blocks) * rank / p.split), kb1 = int(int64_t(p.k_blocks) * (rank + 1) / p.split);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kRing; ++s) {
+        for (int s = 0; s < p.ring; ++s) {
             mbar_init(&sm.full[s], 1);
             mbar_init(&sm.empty[s], 1);
         }
@@ -487,20 +606,23 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = sm.tmem_base;
+    wait_for_inputs();
 
     if (warp == 0) {
         if (lane == 0) {
-            for (int i = 0; i < kb1 - kb0; ++i) {
-                const int s = i % kRing, kb = kb0 + i;
-                if (i >= kRing && !wait(&sm.empty[s], uint32_t(i / kRing - 1) & 1u, abort_flag, p.status, kWaitEmpty)) break;
-                mbar_arrive_expect_tx(&sm.full[s], kTileBytes + Smem::kXBytes);
+            uint32_t s = 0, turn = 0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (turn > 0 && !wait(&sm.empty[s], (turn - 1u) & 1u, abort_flag, p.status, kWaitEmpty)) break;
+                uint8_t* stage = ring + s * kStageBytes;
+                mbar_arrive_expect_tx(&sm.full[s], kStageBytes);
                 if constexpr (W_MN) {
-                    tma_load_4d(sm.ring.w[s], &map_w, &sm.full[s], output0, kb * kBlockK, 0, 0);
-                    tma_load_4d(sm.ring.w[s] + kPanelBytes, &map_w, &sm.full[s], output0 + 64, kb * kBlockK, 0, 0);
+                    tma_load_4d(stage, &map_w, &sm.full[s], output0, kb * kBlockK, 0, 0);
+                    tma_load_4d(stage + kPanelBytes, &map_w, &sm.full[s], output0 + 64, kb * kBlockK, 0, 0);
                 } else {
-                    tma_load_4d(sm.ring.w[s], &map_w, &sm.full[s], kb * kBlockK, output0, 0, 0);
+                    tma_load_4d(stage, &map_w, &sm.full[s], kb * kBlockK, output0, 0, 0);
                 }
-                tma_load_4d(sm.ring.x[s], &map_x, &sm.full[s], kb * kBlockK, token0, 0, 0);
+                tma_load_4d(stage + kTileBytes, &map_x, &sm.full[s], kb * kBlockK, token0, 0, 0);
+                if (++s == uint32_t(p.ring)) s = 0, ++turn;
             }
         }
         __syncwarp();
@@ -508,17 +630,19 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         const bool elected = elect_one();
         constexpr uint32_t idesc = instruction<DT>(128, TOKENS, W_MN, false);
         constexpr uint32_t desc_hi = umma_smem_desc_hi(1024);
+        const uint32_t w_first = tile_lo<W_MN>(ring), x_first = tile_lo<false>(ring + kTileBytes);
+        uint32_t s = 0, turn = 0;
         bool ok = true;
         for (int i = 0; i < kb1 - kb0; ++i) {
-            const int s = i % kRing;
-            ok = wait(&sm.full[s], uint32_t(i / kRing) & 1u, abort_flag, p.status, kWaitFull);
+            ok = wait(&sm.full[s], turn & 1u, abort_flag, p.status, kWaitFull);
             if (!ok) break;
             tc_fence_after_sync();
-            const uint32_t w_lo = tile_lo<W_MN>(sm.ring.w[s]), x_lo = tile_lo<false>(sm.ring.x[s]);
+            const uint32_t w_lo = w_first + s * (kStageBytes / 16u), x_lo = x_first + s * (kStageBytes / 16u);
 #pragma unroll
             for (uint32_t k = 0; k < kBlockK / 16; ++k)
                 if (elected) umma_ss_words(tmem, w_lo + k * kStep16<W_MN>, x_lo + k * kStep16<false>, desc_hi, idesc, (i > 0 || k > 0) ? 1u : 0u);
             if (elected) umma_commit(&sm.empty[s]);
+            if (++s == uint32_t(p.ring)) s = 0, ++turn;
         }
         if (ok && elected) umma_commit(&sm.acc_full);
         __syncwarp();
@@ -535,7 +659,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             tmem_ld_32x32b_x16(tmem + lane_base + uint32_t(c), acc);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sm.partial[c + i][32 * (warp & 3) + lane] = __uint_as_float(acc[i]);
+            for (int i = 0; i < 16; ++i) partial[c + i][32 * (warp & 3) + lane] = __uint_as_float(acc[i]);
         }
     }
     tc_fence_before_sync();
@@ -553,7 +677,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         for (int t = rank * (kSplitThreads / 32) + warp; t < TOKENS && token0 + t < p.m; t += warps) {
             float z[4];
             if (p.split > 1) {
-                const uint32_t mine = smem_u32(&sm.partial[t][4 * lane]);
+                const uint32_t mine = smem_u32(&partial[t][4 * lane]);
                 float4 part[kMaxSplit];
 #pragma unroll
                 for (int r = 0; r < kMaxSplit; ++r)
@@ -563,7 +687,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 for (int r = 1; r < kMaxSplit; ++r)
                     if (r < p.split) z[0] += part[r].x, z[1] += part[r].y, z[2] += part[r].z, z[3] += part[r].w;
             } else {
-                const float4 v = *reinterpret_cast<const float4*>(&sm.partial[t][4 * lane]);
+                const float4 v = *reinterpret_cast<const float4*>(&partial[t][4 * lane]);
                 z[0] = v.x, z[1] = v.y, z[2] = v.z, z[3] = v.w;
             }
             if (output < p.n) finish<DT, 4>(p, z, token0 + t, output);
@@ -654,9 +778,11 @@ __global__ void __launch_bounds__(kActThreads) linear_grad_act_kernel(const Grad
 // the chunks' sums, always in the same order
 __global__ void __launch_bounds__(256) linear_bias_grad_kernel(const float* __restrict__ partial, void* out, int chunks, int n, int dtype) {
     __shared__ float part[8][33];
+    wait_for_inputs();
     const int column = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;
     float sum = 0.0f;
     if (column < n)
+#pragma unroll 4
         for (int c = lane; c < chunks; c += 8) sum += partial[int64_t(c) * n + column];
     part[lane][threadIdx.x & 31] = sum;
     __syncthreads();
@@ -685,40 +811,66 @@ struct Product {
     bool a_mn, b_mn;                   // operand stored [k, rows] instead of [rows, k]
 };
 
-template <class K>
-cudaError_t launch_cluster(K kernel, unsigned grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t stream,
-                           const CUtensorMap& a, const CUtensorMap& b, const LinearParams& p) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-    if (e != cudaSuccess) return e;
+// A launch that may begin while the kernel before it in the stream drains; `cluster` 0: the kernel's own attribute, or none.
+template <class... P, class... A>
+cudaError_t launch_early(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t stream, const A&... args) {
+    if (smem > 48 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+        if (e != cudaSuccess) return e;
+    }
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(grid);
     config.blockDim = dim3(threads);
     config.dynamicSmemBytes = smem;
     config.stream = stream;
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeClusterDimension;
-    attribute.val.clusterDim.x = cluster;
-    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
-    config.attrs = &attribute;
-    config.numAttrs = cluster ? 1 : 0;
-    return cudaLaunchKernelEx(&config, kernel, a, b, p);
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = cluster;
+    attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = cluster ? 2 : 1;
+    return cudaLaunchKernelEx(&config, kernel, P(args)...);
+}
+
+// Columns of an output tile.  A tile's time goes with its width and some 64 columns more (measured, 4096 x 4096 x 14336, us per
+// tile at widths 96, 128 .. 256: 16.6, 17.2, 19.3, 21.7, 24.3, 27.6); the launch takes as many of them as the busiest pair has,
+// but where power is the limit pairs that run dry early leave clock to the others, so that the mean counts half.
+// Measured at 4096 x 4096 x 4096, us at widths 128, 160 .. 256: 123, 113, 101, 100, 96 (3.46 tiles a pair at the last).
+int pair_columns(const Product& q, int pairs) {
+    const int key = fpt::tuning_linear_columns();
+    if (key > 0) return key;
+    const int64_t row_tiles = (q.m + 255) / 256;
+    int best = 256;
+    int64_t least = INT64_MAX;
+    for (int c = 256; c >= 64; c -= 32) {
+        const int64_t tiles = row_tiles * ((q.n + c - 1) / c), rounds = (tiles + pairs - 1) / pairs;
+        const int64_t time = (rounds * pairs + tiles) * (c + 64);
+        if (time < least) {
+            least = time;
+            best = c;
+        }
+    }
+    return best;
 }
 
 template <int DT, bool A_MN, bool B_MN>
 int launch_pair(const Product& q, LinearParams& p, const DeviceInfo& dev, cudaStream_t stream) {
     CUtensorMap map_a, map_b;
     if (int rc = A_MN ? operand_map(&map_a, q.a, q.k, q.m, q.a_ld, kBlockK) : operand_map(&map_a, q.a, q.m, q.k, q.a_ld, 128)) return rc;
-    if (int rc = B_MN ? operand_map(&map_b, q.b, q.k, q.n, q.b_ld, kBlockK) : operand_map(&map_b, q.b, q.n, q.k, q.b_ld, 128)) return rc;
+    p.columns = pair_columns(q, dev.sm_count / 2);
+    if (int rc = B_MN ? operand_map(&map_b, q.b, q.k, q.n, q.b_ld, kBlockK) : operand_map(&map_b, q.b, q.n, q.k, q.b_ld, p.columns / 2)) return rc;
     p.m_tiles = int((q.m + 255) / 256);
-    p.n_tiles = int((q.n + 255) / 256);
+    p.n_tiles = int((q.n + p.columns - 1) / p.columns);
+    p.stage_bytes = kTileBytes + (uint32_t(p.columns / 2) * 128u + 1023u) / 1024u * 1024u;
+    if (B_MN) p.stage_bytes = kTileBytes + (p.columns > 128 ? 2u : 1u) * kPanelBytes;
+    p.ring = int(std::min<uint32_t>(kMaxRing, kRingBytes / p.stage_bytes));
+    p.staged = p.vec_out && (!p.residual || p.vec_res) && (!p.slope || p.vec_slope);
     static_assert(sizeof(PairSmem) + 1024 <= 227 * 1024, "shared memory budget");
     const size_t smem = sizeof(PairSmem) + 1024;
     const int64_t pairs = std::min<int64_t>(int64_t(p.m_tiles) * p.n_tiles, dev.sm_count / 2);
-    auto kernel = linear_pair_kernel<DT, A_MN, B_MN>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-    if (e != cudaSuccess) return int(e);
-    kernel<<<unsigned(2 * pairs), kPairThreads, smem, stream>>>(map_a, map_b, p);
-    return cuda_status(cudaGetLastError());
+    return cuda_status(launch_early(linear_pair_kernel<DT, A_MN, B_MN>, unsigned(2 * pairs), kPairThreads, smem, 0u, stream, map_a, map_b, p));
 }
 
 // B, the tokens' operand, becomes the column side: D is written row by row as [tokens, outputs] all the same
@@ -727,14 +879,17 @@ int launch_split(const Product& q, LinearParams& p, const DeviceInfo& dev, int s
     CUtensorMap map_w, map_x;
     if (int rc = W_MN ? operand_map(&map_w, q.b, q.k, q.n, q.b_ld, kBlockK) : operand_map(&map_w, q.b, q.n, q.k, q.b_ld, 128)) return rc;
     if (int rc = operand_map(&map_x, q.a, q.m, q.k, q.a_ld, TOKENS)) return rc;
-    using Smem = SplitSmem<TOKENS>;
-    static_assert(2 * (sizeof(Smem) + 2048) <= 228 * 1024, "two blocks an SM");
     p.m_tiles = int((q.m + TOKENS - 1) / TOKENS);
     p.n_tiles = int((q.n + 127) / 128);
     p.split = split;
     const int64_t blocks = int64_t(p.m_tiles) * p.n_tiles * split;
     if (blocks > 0x7fffffff) return FPT_ERR_BAD_SIZE;
-    return cuda_status(launch_cluster(linear_split_kernel<DT, TOKENS, W_MN>, unsigned(blocks), kSplitThreads, sizeof(Smem) + 1024,
+    // all the shared memory where every block has an SM to itself, else two blocks an SM
+    const uint32_t stage = kTileBytes + TOKENS * 128;
+    const uint32_t budget = blocks <= dev.sm_count ? 216u * 1024u : 108u * 1024u;
+    p.ring = int(std::min<uint32_t>(kMaxRing, budget / stage));
+    const size_t smem = 1024 + kSplitRingOffset + std::max<size_t>(size_t(p.ring) * stage, size_t(TOKENS) * 512);
+    return cuda_status(launch_early(linear_split_kernel<DT, TOKENS, W_MN>, unsigned(blocks), kSplitThreads, smem,
                                       split > 1 ? unsigned(split) : 0u, stream, map_w, map_x, p));
 }
 
@@ -932,8 +1087,8 @@ extern "C" int fpt_linear_grad_act(void* dz, void* dbias, const void* dy, const 
         if (int rc = cuda_status(cudaGetLastError())) return rc;
     }
     if (dbias) {
-        linear_bias_grad_kernel<<<unsigned((out_features + 31) / 32), 256, 0, stream>>>(static_cast<const float*>(workspace), dbias, chunks, int(out_features), bias_dtype);
-        return cuda_status(cudaGetLastError());
+        return cuda_status(launch_early(linear_bias_grad_kernel, unsigned((out_features + 31) / 32), 256u, 0, 0u, stream,
+                                        static_cast<const float*>(workspace), dbias, chunks, int(out_features), bias_dtype));
     }
     return FPT_OK;
 }

@@ -75,7 +75,8 @@ struct QkRopeArgs {
     int64_t pos_axis, pos_b, pos_s;    // in elements
     int pos_words;                     // 1: 32-bit positions, 2: 64-bit
     Divider seq, pairs, parts;         // parts: blocks that share the heads of a token (forward)
-    uint32_t tokens, tile_tokens;      // tile_tokens: a power of two (forward)
+    uint32_t tokens, tile_tokens;      // tile_tokens: a power of two
+    uint32_t groups;                   // heads a block has in hand at a time (forward)
     uint32_t heads_per_part;
     int dim, units, rotary_units;      // lanes of a head that hold something, that rotate
     float eps;
@@ -434,18 +435,23 @@ __device__ __forceinline__ void keep_weight(float (&weight)[2][kMaxPairs], const
 
 // Lanes that hold nothing (heads that do not fill their group) read what lane 0 reads and count as zeros, and a group past
 // the last head or token reads the last one: no load is predicated.
+// Without the norm nothing passes between the lanes of a head, and groups of exactly as many lanes as hold something (G = 0)
+// leave none idle.
 // The heads of a token are numbered through, queries first.  A block has the heads [head0, head1) of its tokens (all of
-// them where a tile has several tokens); the kGroups / tile_tokens groups of a token take them in turn.
+// them where a tile has several tokens); the groups of a token take them in turn.
 template <class T, int C, int G, bool HALVES, bool NORM>
 __global__ void __launch_bounds__(kThreads, (kFwdBlocks<T, NORM>)) qk_rope_kernel(const __grid_constant__ QkRopeArgs a) {
-    constexpr uint32_t kGroups = kThreads / G, kAhead = kStages - 1;
+    constexpr uint32_t kAhead = kStages - 1;
     extern __shared__ __align__(16) char ring_raw[];
     __shared__ Shared sm;
     const Ring<T, C, kStages> ring(ring_raw);
     const uint32_t tile = a.parts.div(blockIdx.x), part = blockIdx.x - tile * a.parts.d;
     const uint32_t token0 = tile * a.tile_tokens, count = min(a.tile_tokens, a.tokens - token0);
-    const int lane_unit = threadIdx.x & (G - 1);
-    const bool live = lane_unit < a.units;
+    const bool one = a.tile_tokens == 1;
+    const uint32_t group = G ? threadIdx.x / G : threadIdx.x / uint32_t(a.units);
+    const int lane_unit = int(threadIdx.x - group * (G ? G : uint32_t(a.units)));
+    const uint32_t step = a.groups / a.tile_tokens;                                   // groups of a token
+    const bool live = lane_unit < a.units && group < step * a.tile_tokens;
     const int unit = live ? lane_unit : 0;
     const Place at = place<C>(unit, a.rotary_units);
     const uint32_t lo = uint32_t(at.lo) * sizeof(T), hi = uint32_t(at.hi) * sizeof(T), out_bytes = uint32_t(a.dim) * sizeof(T);
@@ -456,8 +462,6 @@ __global__ void __launch_bounds__(kThreads, (kFwdBlocks<T, NORM>)) qk_rope_kerne
         weight[0] = fetch_weight<C, HALVES>(a.side[0], a);
         weight[1] = fetch_weight<C, HALVES>(a.side[1], a);
     }
-    const bool one = a.tile_tokens == 1;
-    const uint32_t step = kGroups / a.tile_tokens, group = threadIdx.x / G;          // groups of a token
     const uint32_t my_slot = group / step, slot = min(my_slot, count - 1);
     const uint32_t q_heads = a.side[0].heads, heads = q_heads + a.side[1].heads;
     const uint32_t head0 = part * a.heads_per_part, head1 = min(head0 + a.heads_per_part, heads);
@@ -844,7 +848,8 @@ extern "C" int fpt_qk_rope(void* q_out, void* k_out, const void* q, const void* 
     a.sin_sign = inverse ? 0x80000000u : 0u;
     // One head per group and block while that gives no more than a few blocks per SM (single tokens: the shortest chain
     // of loads); beyond it a block takes all heads of as many tokens as leave every group at least four heads.
-    const uint32_t groups = uint32_t(kThreads / group_lanes(a.units)), heads = a.side[0].heads + a.side[1].heads;
+    const uint32_t groups = uint32_t(kThreads / (norm ? group_lanes(a.units) : a.units)), heads = a.side[0].heads + a.side[1].heads;
+    a.groups = groups;
     const bool few = uint64_t(a.tokens) * heads <= uint64_t(groups) * uint64_t(dev.sm_count) * 4;
     a.tile_tokens = few ? 1u : tile_tokens(groups, heads, uint32_t(pairs), 4, kMaxTrig);
     for (const Side& s : a.side)
@@ -858,7 +863,7 @@ extern "C" int fpt_qk_rope(void* q_out, void* k_out, const void* q, const void* 
         constexpr int C = decltype(c)::value, G = decltype(g)::value;
         constexpr bool H = decltype(halves)::value;
         return norm ? launch(qk_rope_kernel<T, C, G, H, true>, grid, Ring<T, C, kStages>::kBytes, stream, a)
-                    : launch(qk_rope_kernel<T, C, G, H, false>, grid, Ring<T, C, kStages>::kBytes, stream, a);
+                    : launch(qk_rope_kernel<T, C, 0, H, false>, grid, Ring<T, C, kStages>::kBytes, stream, a);
     });
 }
 

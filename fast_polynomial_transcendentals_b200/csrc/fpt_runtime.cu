@@ -27,6 +27,7 @@ std::atomic<int> g_gate_up_cta_pair{-1};
 std::atomic<int> g_gate_up_pair_wide{0};
 std::atomic<int> g_linear_tokens{-1};
 std::atomic<int> g_linear_split{0};
+std::atomic<int> g_linear_columns{0};
 std::atomic<int> g_rope_heads_per_block{8};   // measured: 8 is 1.5-3 % ahead of "all heads in one block" at 32 heads
 
 enum { DT_FP16 = kFp16, DT_BF16 = kBf16 };
@@ -77,6 +78,7 @@ int tuning_attention_cta_pair() { return g_attention_cta_pair.load(); }
 int tuning_gate_up_cta_pair() { return g_gate_up_cta_pair.load(); }
 int tuning_gate_up_pair_wide() { return g_gate_up_pair_wide.load(); }
 int tuning_linear_tokens() { return g_linear_tokens.load(); }
+int tuning_linear_columns() { return g_linear_columns.load(); }
 int tuning_linear_split() { return g_linear_split.load(); }
 int tuning_rope_heads_per_block() { return g_rope_heads_per_block.load(); }
 
@@ -167,6 +169,7 @@ int fpt_set_tuning(const char* key, int value) {
     if (!std::strcmp(key, "attention_cta_pair")) { if (value < 0 || value > 1) return FPT_ERR_BAD_SIZE; fpt::g_attention_cta_pair = value; return FPT_OK; }
     if (!std::strcmp(key, "gate_up_pair_wide")) { if (value < 0 || value > 1) return FPT_ERR_BAD_SIZE; fpt::g_gate_up_pair_wide = value; return FPT_OK; }
     if (!std::strcmp(key, "linear_tokens")) { if (value != -1 && value != 0 && value != 16 && value != 32 && value != 64 && value != 128) return FPT_ERR_BAD_SIZE; fpt::g_linear_tokens = value; return FPT_OK; }
+    if (!std::strcmp(key, "linear_columns")) { if (value != 0 && (value < 64 || value > 256 || value % 32)) return FPT_ERR_BAD_SIZE; fpt::g_linear_columns = value; return FPT_OK; }
     if (!std::strcmp(key, "linear_split")) { if (value < 0 || value > 8) return FPT_ERR_BAD_SIZE; fpt::g_linear_split = value; return FPT_OK; }
     if (!std::strcmp(key, "gate_up_cta_pair")) { if (value < -1 || value > 1) return FPT_ERR_BAD_SIZE; fpt::g_gate_up_cta_pair = value; return FPT_OK; }
     return FPT_ERR_BAD_ENUM;
@@ -184,6 +187,7 @@ int fpt_get_tuning(const char* key, int* value) {
     if (!std::strcmp(key, "attention_cta_pair")) { *value = fpt::g_attention_cta_pair; return FPT_OK; }
     if (!std::strcmp(key, "gate_up_pair_wide")) { *value = fpt::g_gate_up_pair_wide; return FPT_OK; }
     if (!std::strcmp(key, "linear_tokens")) { *value = fpt::g_linear_tokens; return FPT_OK; }
+    if (!std::strcmp(key, "linear_columns")) { *value = fpt::g_linear_columns; return FPT_OK; }
     if (!std::strcmp(key, "linear_split")) { *value = fpt::g_linear_split; return FPT_OK; }
     if (!std::strcmp(key, "gate_up_cta_pair")) { *value = fpt::g_gate_up_cta_pair; return FPT_OK; }
     return FPT_ERR_BAD_ENUM;

@@ -75,6 +75,7 @@ def test_c_abi_checks_before_launch(fpt):
 
 def test_tuning_keys(fpt):
     lib = fpt.load()
-    for key, good, bad in ((b"linear_tokens", (0, 16, 32, 64, 128, -1), (8, 256, -2)), (b"linear_split", (1, 8, 0), (9, -1))):
+    for key, good, bad in ((b"linear_tokens", (0, 16, 32, 64, 128, -1), (8, 256, -2)), (b"linear_split", (1, 8, 0), (9, -1)),
+                           (b"linear_columns", (64, 96, 256, 0), (32, 100, 288, -1))):
         assert all(lib.fpt_set_tuning(key, v) == -2 for v in bad)
         assert all(lib.fpt_set_tuning(key, v) == 0 for v in good)         # the last one is the default

@@ -29,8 +29,9 @@ ACTIVATIONS = ["none", "sigmoid", "tanh", "silu", "gelu"]
 def tuning(fpt):
     lib = fpt.load()
 
-    def set_form(tokens=-1, split=0):
-        assert lib.fpt_set_tuning(b"linear_tokens", tokens) == 0 and lib.fpt_set_tuning(b"linear_split", split) == 0
+    def set_form(tokens=-1, split=0, columns=0):
+        for key, value in ((b"linear_tokens", tokens), (b"linear_split", split), (b"linear_columns", columns)):
+            assert lib.fpt_set_tuning(key, value) == 0
     yield set_form
     set_form()
 
@@ -129,6 +130,14 @@ def test_every_form(cuda, tuning, tokens, shape):
     for split in ([1, 2, 3, 5, 8] if tokens else [0]):
         tuning(tokens, split)
         check(*args, "gelu", what=f"tokens {tokens} split {split}")
+    check_linear_status()
+
+
+@pytest.mark.parametrize("columns", range(64, 257, 32))
+def test_every_tile_width(cuda, tuning, columns):
+    for shape in ((300, 200, 520), (70, 136, 1003)):
+        tuning(0, 0, columns)
+        check(*inputs(*shape, torch.bfloat16, cuda), "gelu", what=f"columns {columns}")
     check_linear_status()
 
 
