@@ -47,10 +47,9 @@ constexpr int kMaxRing = 12;                        // stages of a ring
 constexpr int kBandTiles = 16;                      // 256-row tiles per band: 4096 rows, see fpt_gate_up_swiglu.cu
 
 enum : uint32_t { kWaitEmpty = 0x51, kWaitFull, kWaitAccEmpty, kWaitAccFull };
-enum ActKind : int { kActNone, kActNative, kActProgram };
+enum Act : int { kNone, kSigmoid, kTanh, kSwishAct, kGelu, kProgram };   // compile-time: one straight piece of code each
 
-struct Activation {
-    int kind, fn;
+struct Programs {                      // of kProgram
     int fwd_shape, fwd_degree, bwd_shape, bwd_degree;
     ProgramWords fwd, bwd;
 };
@@ -61,16 +60,18 @@ struct LinearParams {
     const void* bias;               // [n] or null
     uint16_t* slope;                // [m, n] fp16 or null
     int64_t out_ld, res_ld, slope_ld;
-    int m, n, k_blocks;
+    int m, n, k_blocks;             // k_blocks: of 64 (split form), of 64 chunks (pair form)
     int m_tiles, n_tiles;
     int split;                      // blocks per cluster (split form)
     int columns;                    // columns of an output tile (pair form), a multiple of 32
-    int ring;                       // stages of the ring and their size (pair form)
-    uint32_t stage_bytes;
+    int ring;                       // stages of the ring
+    uint32_t stage_bytes;           // their size, and the K blocks of 64 in one (pair form)
+    int chunks;
+    bool a_whole, b_whole;          // one copy brings an operand's share of a stage (pair form)
     int bias_dtype;
     bool vec_out, vec_res, vec_slope, vec_bias;
     bool staged;                    // out, residual and slope rows all start on 16-byte boundaries (pair form)
-    Activation act;
+    Programs act;
     uint32_t* status;
 };
 
@@ -122,60 +123,65 @@ __device__ __forceinline__ uint32_t run_program(uint32_t x, const ProgramWords& 
     return P::fma(x & ~kSignMask, h, P::mul(Consts<DT>::half, x));       // kSwish
 }
 
+// P(Z > a) for a standard normal Z and a >= 0, with e = exp(-a^2 / 2): Abramowitz and Stegun 7.1.26 (erf to 1.5e-7) at a / sqrt 2
+__device__ __forceinline__ float normal_tail(float a, float e) {
+    const float t = mufu_rcp(fmaf(a, 0.23164189f, 1.0f));                                 // 0.3275911 / sqrt 2
+    float q = fmaf(t, 0.5307027145f, -0.7265760135f);
+    q = fmaf(t, q, 0.7107068705f);
+    q = fmaf(t, q, -0.142248368f);
+    q = fmaf(t, q, 0.127414796f);
+    return q * t * e;
+}
+// tanh: the quotient of exponentials, and where that cancels (|z| < 0.3) its series to z^9 (next term < 2^-24 of z)
+__device__ __forceinline__ float tanh_of(float z) {
+    const float far = fmaf(-2.0f, mufu_rcp(1.0f + mufu_ex2(2.8853900817779268f * z)), 1.0f);
+    const float q = z * z;
+    float s = fmaf(q, 2.1869488536e-2f, -5.3968253968e-2f);
+    s = fmaf(q, s, 1.3333333333e-1f);
+    s = fmaf(q, s, -3.3333333333e-1f);
+    return fabsf(z) < 0.3f ? fmaf(z * q, s, z) : far;
+}
 __device__ __forceinline__ float logistic(float z) { return mufu_rcp(1.0f + mufu_ex2(-1.4426950408889634f * z)); }
 
 // z -> act(z), d -> act'(z) where wanted
-template <int DT, int N>
-__device__ __forceinline__ void activate(const Activation& a, float (&z)[N], float (&d)[N], bool want) {
-    if (a.kind == kActNone) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) d[i] = 1.0f;
-    } else if (a.kind == kActProgram) {
+template <int DT, int ACT, bool SLOPE, int N>
+__device__ __forceinline__ void activate(const Programs& a, float (&z)[N], float (&d)[N]) {
+    if constexpr (ACT == kProgram) {
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
             const uint32_t x = Sfu<DT>::pack(z[i], z[i + 1]);
             const uint32_t y = run_program<DT>(x, a.fwd, a.fwd_shape, a.fwd_degree);
             z[i] = Sfu<DT>::lo(y);
             z[i + 1] = Sfu<DT>::hi(y);
-            if (want) {
+            if constexpr (SLOPE) {
                 const uint32_t s = run_program<DT>(x, a.bwd, a.bwd_shape, a.bwd_degree);
                 d[i] = Sfu<DT>::lo(s);
                 d[i + 1] = Sfu<DT>::hi(s);
             }
         }
-    } else if (a.fn == FPT_FN_GELU) {
+    } else if constexpr (ACT != kNone) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const float x = z[i], phi = 0.5f * (1.0f + erff(x * 0.70710678118654752440f));
-            z[i] = x * phi;
-            if (want) d[i] = fmaf(x * 0.3989422804014327f, mufu_ex2(-0.72134752044448170368f * x * x), phi);
-        }
-    } else if (a.fn == FPT_FN_SWISH) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float x = z[i], p = logistic(x);
-            z[i] = x * p;
-            if (want) d[i] = p * fmaf(x, 1.0f - p, 1.0f);
-        }
-    } else if (a.fn == FPT_FN_SIGMOID) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float p = logistic(z[i]);
-            z[i] = p;
-            if (want) d[i] = p * (1.0f - p);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float y = tanhf(z[i]);
-            z[i] = y;
-            if (want) d[i] = fmaf(-y, y, 1.0f);
+            const float x = z[i];
+            if constexpr (ACT == kGelu) {
+                const float e = mufu_ex2(-0.72134752044448170368f * x * x), tail = normal_tail(fabsf(x), e);
+                const float phi = x < 0.0f ? tail : 1.0f - tail;
+                z[i] = x * phi;
+                if constexpr (SLOPE) d[i] = fmaf(x * 0.3989422804014327f, e, phi);
+            } else if constexpr (ACT == kTanh) {
+                z[i] = tanh_of(x);
+                if constexpr (SLOPE) d[i] = fmaf(-z[i], z[i], 1.0f);
+            } else {
+                const float q = logistic(x);
+                z[i] = ACT == kSwishAct ? x * q : q;
+                if constexpr (SLOPE) d[i] = ACT == kSwishAct ? q * fmaf(x, 1.0f - q, 1.0f) : q * (1.0f - q);
+            }
         }
     }
 }
 
 // N consecutive columns of one row: bias, activation, residual, stores.  N is a multiple of 4; column a multiple of N.
-template <int DT, int N>
+template <int DT, int ACT, bool SLOPE, int N>
 __device__ __forceinline__ void finish(const LinearParams& p, float (&z)[N], int row, int column) {
     constexpr int kWords = N / 2, kVec = kWords >= 4 ? 4 : 2;            // 16-byte accesses, 8-byte ones for N = 4
     using V = std::conditional_t<kVec == 4, uint4, uint2>;
@@ -206,8 +212,8 @@ __device__ __forceinline__ void finish(const LinearParams& p, float (&z)[N], int
         }
     }
     float d[N];
-    activate<DT, N>(p.act, z, d, p.slope != nullptr);
-    if (p.slope) {
+    activate<DT, ACT, SLOPE>(p.act, z, d);
+    if constexpr (SLOPE) {
         uint16_t* to = p.slope + int64_t(row) * p.slope_ld + column;
         if (whole && p.vec_slope) {
 #pragma unroll
@@ -293,42 +299,35 @@ __device__ __forceinline__ void stage_to_rows(const Stage& s, uint16_t* base, in
     }
 }
 
-// All 32 lanes, converged.  `res`: this chunk of the residual as load_rows left it (where p.residual).
-template <int DT>
-__device__ __forceinline__ void finish_staged(const LinearParams& p, float (&z)[32], const uint4 (&res)[4], Stage& s, int row0, int column, int lane) {
+// All 32 lanes, converged.  `res`: this chunk of the residual as load_rows left it (where p.residual); `bias`: of column
+// `column + lane` (where p.bias).
+template <int DT, int ACT, bool SLOPE>
+__device__ __forceinline__ void finish_staged(const LinearParams& p, float (&z)[32], const uint4 (&res)[4], float bias, Stage& s, int row0, int column, int lane) {
     const int valid = p.m - row0;
-    if (p.bias) {
-        if (p.bias_dtype != FPT_FP32 && p.vec_bias) {
-            const uint4* b = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.bias) + column);
+    if (p.bias) {                                   // a column per lane, read back by all
+        float* shared = reinterpret_cast<float*>(s.piece);
+        shared[lane] = bias;
+        __syncwarp();
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const uint4 q = b[v];
-                const uint32_t words[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool bf = p.bias_dtype == FPT_BF16;
-                    z[8 * v + 2 * i] += bf ? Sfu<kBf16>::lo(words[i]) : Sfu<kFp16>::lo(words[i]);
-                    z[8 * v + 2 * i + 1] += bf ? Sfu<kBf16>::hi(words[i]) : Sfu<kFp16>::hi(words[i]);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) z[i] += load_any(p.bias, p.bias_dtype, column + i);
+        for (int i = 0; i < 8; ++i) {
+            const float4 v = reinterpret_cast<const float4*>(shared)[i];
+            z[4 * i] += v.x, z[4 * i + 1] += v.y, z[4 * i + 2] += v.z, z[4 * i + 3] += v.w;
         }
+        __syncwarp();
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {                   // halves: fewer registers
         float (&half)[16] = *reinterpret_cast<float (*)[16]>(z + 16 * h);
         float d[16];
-        activate<DT, 16>(p.act, half, d, p.slope != nullptr);
-        if (p.slope) {
+        activate<DT, ACT, SLOPE>(p.act, half, d);
+        if constexpr (SLOPE) {
 #pragma unroll
             for (int q = 0; q < 2; ++q)
                 s.piece[stage_at(lane, 2 * h + q)] = make_uint4(Sfu<kFp16>::pack(d[8 * q], d[8 * q + 1]), Sfu<kFp16>::pack(d[8 * q + 2], d[8 * q + 3]),
                                                                 Sfu<kFp16>::pack(d[8 * q + 4], d[8 * q + 5]), Sfu<kFp16>::pack(d[8 * q + 6], d[8 * q + 7]));
         }
     }
-    if (p.slope) {
+    if constexpr (SLOPE) {
         __syncwarp();
         stage_to_rows(s, p.slope + int64_t(row0) * p.slope_ld + column, p.slope_ld, lane, valid);
         __syncwarp();
@@ -371,14 +370,19 @@ constexpr uint32_t kStep16 = MN ? 2048u / 16u : 2u;
 // ---- many rows: pairs of CTAs ---------------------------------------------------------------------------------------
 
 constexpr uint32_t kRingBytes = 192 * 1024;
-constexpr int kPairThreads = 384;       // TMA, product and allocation warps, one idle, eight epilogue warps
+constexpr int kChunks = 2;              // K blocks of 64 in a stage
+// TMA, product and allocation warps, one idle, eight epilogue warps.  Measured (1999 x 1408 x 2048 fp16, one tile a pair, SiLU,
+// bias and residual): 17.3 us with eight, 17.4 with twelve, 18.4 with sixteen (96 registers a thread, spills); one epilogue for
+// all activations, chosen at run time, took 23.4.
+constexpr int kEpilogueWarps = 8;
+constexpr int kPairThreads = 128 + 32 * kEpilogueWarps;
 
 struct PairSmem {
     alignas(1024) uint8_t ring[kRingBytes];        // stages of an A tile and a B tile, as many as fit
     alignas(8) uint64_t full[kMaxRing];
     uint64_t empty[kMaxRing];
     uint64_t acc_full[2], acc_empty[2];
-    Stage stage[8];
+    Stage stage[kEpilogueWarps];
     uint32_t tmem_base;
     uint32_t abort_flag;
 };
@@ -396,20 +400,42 @@ __device__ __forceinline__ PairTile pair_tile(const LinearParams& p, int tile) {
     return PairTile{(band * kBandTiles + r - column * in_band) * 256, column * p.columns};
 }
 
+// An operand's share of a stage: `rows` rows (at most 128) x 64 chunks K.  K-major: a tile [rows x 64] per chunk; MN-major: a
+// panel [64 chunks k x 64 rows] per 64 rows.  A copy takes the engine some 200 clocks whatever its size (measured: loads
+// alone run at 231-273 ns per K block with two copies in it, 20 or 32 KB alike), so where the sizes allow (`whole`) one copy
+// brings all tiles or panels, through a map whose third dimension walks over them.
 template <bool MN>
-__device__ __forceinline__ void load_pair(uint8_t* tile, const CUtensorMap* map, uint32_t bar, int kb, int row, bool both) {
+__device__ __forceinline__ void load_pair(uint8_t* to, const CUtensorMap* map, uint32_t bar, int kb, int row, int rows, int chunks, bool whole) {
     if constexpr (MN) {
-        tma_load_4d_pair(tile, map, bar, row, kb * kBlockK, 0, 0);
-        if (both) tma_load_4d_pair(tile + kPanelBytes, map, bar, row + 64, kb * kBlockK, 0, 0);
+        if (whole) {
+            tma_load_4d_pair(to, map, bar, 0, kb * chunks * kBlockK, row / 64, 0);
+        } else {
+            tma_load_4d_pair(to, map, bar, row, kb * chunks * kBlockK, 0, 0);
+            if (rows > 64) tma_load_4d_pair(to + uint32_t(chunks) * kPanelBytes, map, bar, row + 64, kb * chunks * kBlockK, 0, 0);
+        }
     } else {
-        tma_load_4d_pair(tile, map, bar, kb * kBlockK, row, 0, 0);
+        if (whole) {
+            tma_load_4d_pair(to, map, bar, 0, row, kb * chunks, 0);
+        } else {
+            for (int c = 0; c < chunks; ++c) tma_load_4d_pair(to + uint32_t(c * rows) * 128u, map, bar, (kb * chunks + c) * kBlockK, row, 0, 0);
+        }
     }
+}
+// shared memory of that share
+template <bool MN>
+__host__ __device__ constexpr uint32_t share_bytes(int rows, int chunks) {
+    return MN ? uint32_t((rows + 63) / 64) * uint32_t(chunks) * kPanelBytes : uint32_t(rows * chunks) * 128u;
+}
+// low word of its descriptor at K step k of 16
+template <bool MN>
+__device__ __forceinline__ uint32_t share_lo(uint32_t first, uint32_t k, uint32_t rows) {
+    return MN ? first + k * (2048u / 16u) : first + k / 4 * (rows * 8u) + k % 4 * 2u;
 }
 
 // Each CTA of the pair holds 128 rows of A and half the tile's columns' rows of B and receives 128 rows x p.columns columns of
 // D; the hand-overs are those of gate_up_swiglu_pair_kernel.  The host picks the number of columns so that the tiles come
 // out even over the pairs.
-template <int DT, bool A_MN, bool B_MN>
+template <int DT, int ACT, bool SLOPE, bool A_MN, bool B_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ LinearParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -424,7 +450,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&sm.acc_full[a], 1);
-            mbar_init(&sm.acc_empty[a], 16);            // eight epilogue warps in each CTA
+            mbar_init(&sm.acc_empty[a], 2 * kEpilogueWarps);   // of both CTAs
         }
         sm.abort_flag = 0u;
         mbar_fence_init();
@@ -448,7 +474,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             uint32_t s = 0, turn = 0;                       // stage, and how often the ring has gone round
             bool ok = true;
             const int b_rows = p.columns / 2;
-            const uint32_t bytes = 2 * (kTileBytes + (B_MN ? (b_rows > 64 ? 2u : 1u) * kPanelBytes : uint32_t(b_rows) * 128u));
+            const uint32_t a_bytes = share_bytes<A_MN>(128, p.chunks), bytes = 2 * (a_bytes + share_bytes<B_MN>(b_rows, p.chunks));
             for (int tile = first_tile; tile < tiles && ok; tile += tile_step) {
                 const PairTile t = pair_tile(p, tile);
                 for (int kb = 0; kb < p.k_blocks; ++kb) {
@@ -457,8 +483,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                     const uint32_t bar = map_to_cta(smem_u32(&sm.full[s]), 0);
                     uint8_t* stage = sm.ring + s * p.stage_bytes;
                     if (rank == 0) mbar_arrive_expect_tx(&sm.full[s], bytes);
-                    load_pair<A_MN>(stage, &map_a, bar, kb, t.row0 + int(rank) * 128, true);
-                    load_pair<B_MN>(stage + kTileBytes, &map_b, bar, kb, t.column0 + int(rank) * b_rows, b_rows > 64);
+                    load_pair<A_MN>(stage, &map_a, bar, kb, t.row0 + int(rank) * 128, 128, p.chunks, p.a_whole);
+                    load_pair<B_MN>(stage + a_bytes, &map_b, bar, kb, t.column0 + int(rank) * b_rows, b_rows, p.chunks, p.b_whole);
                     if (++s == uint32_t(p.ring)) s = 0, ++turn;
                 }
             }
@@ -467,7 +493,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         const bool elected = elect_one();
         const uint32_t idesc = instruction<DT>(256, uint32_t(p.columns), A_MN, B_MN);
         constexpr uint32_t desc_hi = umma_smem_desc_hi(1024);
-        const uint32_t a_first = tile_lo<A_MN>(sm.ring), b_first = tile_lo<B_MN>(sm.ring + kTileBytes);
+        const uint32_t panel = uint32_t(p.chunks) * kPanelBytes, b_rows = uint32_t(p.columns / 2);
+        const uint32_t a_first = umma_smem_desc_lo(smem_u32(sm.ring), A_MN ? panel : 16u);
+        const uint32_t b_first = umma_smem_desc_lo(smem_u32(sm.ring) + share_bytes<A_MN>(128, p.chunks), B_MN ? panel : 16u);
         uint32_t s = 0, turn = 0, local = 0;
         bool ok = true;
         for (int tile = first_tile; tile < tiles && ok; tile += tile_step, ++local) {
@@ -485,17 +513,17 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 if (!ok) break;
                 tc_fence_after_sync();
                 const uint32_t a_lo = a_first + s * (p.stage_bytes / 16u), b_lo = b_first + s * (p.stage_bytes / 16u);
-#pragma unroll
-                for (uint32_t k = 0; k < kBlockK / 16; ++k)
-                    if (elected) umma_ss_words_pair(tmem + a * 256u, a_lo + k * kStep16<A_MN>, b_lo + k * kStep16<B_MN>, desc_hi, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+#pragma unroll 4
+                for (uint32_t k = 0; k < uint32_t(p.chunks) * (kBlockK / 16); ++k)
+                    if (elected) umma_ss_words_pair(tmem + a * 256u, share_lo<A_MN>(a_lo, k, 128), share_lo<B_MN>(b_lo, k, b_rows), desc_hi, idesc, (kb > 0 || k > 0) ? 1u : 0u);
                 if (elected) umma_commit_pair(&sm.empty[s], 3);
                 if (++s == uint32_t(p.ring)) s = 0, ++turn;
             }
             if (ok && elected) umma_commit_pair(&sm.acc_full[a], 3);
         }
     } else if (warp >= 4) {
-        // four warps hold the 128 rows (a warp reads the 32 lanes of its number modulo 4); two such sets take the 32-column
-        // chunks in turn
+        // four warps hold the 128 rows (a warp reads the 32 lanes of its number modulo 4); such sets take the 32-column chunks in
+        // turn
         const uint32_t lane_base = uint32_t(32 * (warp & 3)) << 16;
         const int set = (warp - 4) >> 2;
         Stage& stage = sm.stage[warp - 4];
@@ -507,16 +535,18 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             const int row0 = t.row0 + int(rank) * 128 + 32 * (warp & 3), valid = p.m - row0;
             const int column_end = min(p.n, t.column0 + p.columns);
             uint4 res[4];
-            const auto prefetch = [&](int column) {                     // the residual of a chunk, ahead of its turn
-                if (p.residual && p.staged && column + 32 <= column_end && valid > 0)
-                    load_rows(res, static_cast<const uint16_t*>(p.residual) + int64_t(row0) * p.res_ld + column, p.res_ld, lane, valid);
+            float bias = 0.0f;
+            const auto prefetch = [&](int column) {                     // residual and bias of a chunk, ahead of its turn
+                if (!p.staged || column + 32 > column_end || valid <= 0) return;
+                if (p.residual) load_rows(res, static_cast<const uint16_t*>(p.residual) + int64_t(row0) * p.res_ld + column, p.res_ld, lane, valid);
+                if (p.bias) bias = load_any(p.bias, p.bias_dtype, column + lane);
             };
             prefetch(t.column0 + set * 32);
             ok = wait(&sm.acc_full[a], (local >> 1) & 1u, abort_flag, p.status, kWaitAccFull);
             if (!ok) break;
             tc_fence_after_sync();
 #pragma unroll 1
-            for (int c = set * 32; c < p.columns; c += 64) {
+            for (int c = set * 32; c < p.columns; c += kEpilogueWarps * 8) {
                 const int column = t.column0 + c;
                 if (column >= p.n || valid <= 0) break;
                 uint32_t acc[32];
@@ -526,11 +556,12 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 #pragma unroll
                 for (int i = 0; i < 32; ++i) z[i] = __uint_as_float(acc[i]);
                 if (p.staged && column + 32 <= p.n) {
-                    uint4 mine[4] = {res[0], res[1], res[2], res[3]};
-                    prefetch(column + 64);
-                    finish_staged<DT>(p, z, mine, stage, row0, column, lane);
+                    const uint4 mine[4] = {res[0], res[1], res[2], res[3]};
+                    const float mine_bias = bias;
+                    prefetch(column + kEpilogueWarps * 8);
+                    finish_staged<DT, ACT, SLOPE>(p, z, mine, mine_bias, stage, row0, column, lane);
                 } else {
-                    if (lane < valid) finish<DT, 32>(p, z, row0 + lane, column);
+                    if (lane < valid) finish<DT, ACT, SLOPE>(p, z, row0 + lane, column);
                     __syncwarp();
                 }
             }
@@ -573,7 +604,7 @@ __device__ __forceinline__ float4 load_cluster(uint32_t address) {
 
 // D is [tokens, outputs] (p.m tokens, p.n outputs); A = the weight, B = the tokens.  The p.split blocks of a cluster take
 // equal runs of K blocks.
-template <int DT, int TOKENS, bool W_MN>
+template <int DT, int ACT, bool SLOPE, int TOKENS, bool W_MN>
 __global__ void __launch_bounds__(kSplitThreads, 2)
 linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ LinearParams p) {
     constexpr uint32_t kXBytes = TOKENS * 128, kStageBytes = kTileBytes + kXBytes;
@@ -690,7 +721,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 const float4 v = *reinterpret_cast<const float4*>(&partial[t][4 * lane]);
                 z[0] = v.x, z[1] = v.y, z[2] = v.z, z[3] = v.w;
             }
-            if (output < p.n) finish<DT, 4>(p, z, token0 + t, output);
+            if (output < p.n) finish<DT, ACT, SLOPE>(p, z, token0 + t, output);
         }
     }
     if (p.split > 1) {                            // the partial sums stay until the whole cluster has read them
@@ -804,6 +835,20 @@ int operand_map(CUtensorMap* map, const void* base, int64_t rows, int64_t column
     const uint64_t strides[3] = {uint64_t(ld) * 2, plane, plane};
     return make_tensor_map_bf16_4d(map, base, dims, strides, uint32_t(box_rows));
 }
+// the same with the columns as columns / 64 slices: boxes of 64 columns x box_rows x box_slices.  Only for whole slices: a
+// slice that reached past the row's end would read the next row's values, and past the last row's end other memory.
+int sliced_map(CUtensorMap* map, const void* base, int64_t rows, int64_t columns, int64_t ld, int box_rows, int box_slices) {
+    const uint64_t dims[4] = {64, uint64_t(rows), uint64_t(columns / 64), 1};
+    const uint64_t strides[3] = {uint64_t(ld) * 2, 128, uint64_t(ld) * 2 * uint64_t(rows)};
+    return make_tensor_map_bf16_4d(map, base, dims, strides, uint32_t(box_rows), uint32_t(box_slices));
+}
+// one operand of the pair form, `size` of its rows per CTA and tile
+// (an MN-major operand in slices starts its tiles on slices)
+int pair_map(CUtensorMap* map, bool* whole, const void* base, int64_t rows, int64_t k, int64_t ld, bool mn, int size, int chunks) {
+    *whole = mn ? rows % 64 == 0 && size % 64 == 0 : k % 64 == 0;
+    if (mn) return *whole ? sliced_map(map, base, k, rows, ld, chunks * kBlockK, size > 64 ? 2 : 1) : operand_map(map, base, k, rows, ld, chunks * kBlockK);
+    return *whole ? sliced_map(map, base, rows, k, ld, size, chunks) : operand_map(map, base, rows, k, ld, size);
+}
 
 struct Product {
     const void *a, *b;                 // D[i, j] = sum_k A[i, k] B[j, k], i < m, j < n
@@ -845,6 +890,7 @@ int pair_columns(const Product& q, int pairs) {
     int best = 256;
     int64_t least = INT64_MAX;
     for (int c = 256; c >= 64; c -= 32) {
+        if (q.b_mn && c % 128) continue;            // whole slices of 64 columns for either CTA of the pair
         const int64_t tiles = row_tiles * ((q.n + c - 1) / c), rounds = (tiles + pairs - 1) / pairs;
         const int64_t time = (rounds * pairs + tiles) * (c + 64);
         if (time < least) {
@@ -855,26 +901,27 @@ int pair_columns(const Product& q, int pairs) {
     return best;
 }
 
-template <int DT, bool A_MN, bool B_MN>
+template <int DT, int ACT, bool SLOPE, bool A_MN, bool B_MN>
 int launch_pair(const Product& q, LinearParams& p, const DeviceInfo& dev, cudaStream_t stream) {
     CUtensorMap map_a, map_b;
-    if (int rc = A_MN ? operand_map(&map_a, q.a, q.k, q.m, q.a_ld, kBlockK) : operand_map(&map_a, q.a, q.m, q.k, q.a_ld, 128)) return rc;
     p.columns = pair_columns(q, dev.sm_count / 2);
-    if (int rc = B_MN ? operand_map(&map_b, q.b, q.k, q.n, q.b_ld, kBlockK) : operand_map(&map_b, q.b, q.n, q.k, q.b_ld, p.columns / 2)) return rc;
+    p.chunks = kChunks;
+    p.k_blocks = int((q.k + p.chunks * kBlockK - 1) / (p.chunks * kBlockK));
+    if (int rc = pair_map(&map_a, &p.a_whole, q.a, q.m, q.k, q.a_ld, A_MN, 128, p.chunks)) return rc;
+    if (int rc = pair_map(&map_b, &p.b_whole, q.b, q.n, q.k, q.b_ld, B_MN, p.columns / 2, p.chunks)) return rc;
     p.m_tiles = int((q.m + 255) / 256);
     p.n_tiles = int((q.n + p.columns - 1) / p.columns);
-    p.stage_bytes = kTileBytes + (uint32_t(p.columns / 2) * 128u + 1023u) / 1024u * 1024u;
-    if (B_MN) p.stage_bytes = kTileBytes + (p.columns > 128 ? 2u : 1u) * kPanelBytes;
+    p.stage_bytes = share_bytes<A_MN>(128, p.chunks) + share_bytes<B_MN>(p.columns / 2, p.chunks);
     p.ring = int(std::min<uint32_t>(kMaxRing, kRingBytes / p.stage_bytes));
     p.staged = p.vec_out && (!p.residual || p.vec_res) && (!p.slope || p.vec_slope);
     static_assert(sizeof(PairSmem) + 1024 <= 227 * 1024, "shared memory budget");
     const size_t smem = sizeof(PairSmem) + 1024;
     const int64_t pairs = std::min<int64_t>(int64_t(p.m_tiles) * p.n_tiles, dev.sm_count / 2);
-    return cuda_status(launch_early(linear_pair_kernel<DT, A_MN, B_MN>, unsigned(2 * pairs), kPairThreads, smem, 0u, stream, map_a, map_b, p));
+    return cuda_status(launch_early(linear_pair_kernel<DT, ACT, SLOPE, A_MN, B_MN>, unsigned(2 * pairs), kPairThreads, smem, 0u, stream, map_a, map_b, p));
 }
 
 // B, the tokens' operand, becomes the column side: D is written row by row as [tokens, outputs] all the same
-template <int DT, int TOKENS, bool W_MN>
+template <int DT, int ACT, bool SLOPE, int TOKENS, bool W_MN>
 int launch_split(const Product& q, LinearParams& p, const DeviceInfo& dev, int split, cudaStream_t stream) {
     CUtensorMap map_w, map_x;
     if (int rc = W_MN ? operand_map(&map_w, q.b, q.k, q.n, q.b_ld, kBlockK) : operand_map(&map_w, q.b, q.n, q.k, q.b_ld, 128)) return rc;
@@ -889,35 +936,35 @@ int launch_split(const Product& q, LinearParams& p, const DeviceInfo& dev, int s
     const uint32_t budget = blocks <= dev.sm_count ? 216u * 1024u : 108u * 1024u;
     p.ring = int(std::min<uint32_t>(kMaxRing, budget / stage));
     const size_t smem = 1024 + kSplitRingOffset + std::max<size_t>(size_t(p.ring) * stage, size_t(TOKENS) * 512);
-    return cuda_status(launch_early(linear_split_kernel<DT, TOKENS, W_MN>, unsigned(blocks), kSplitThreads, smem,
+    return cuda_status(launch_early(linear_split_kernel<DT, ACT, SLOPE, TOKENS, W_MN>, unsigned(blocks), kSplitThreads, smem,
                                       split > 1 ? unsigned(split) : 0u, stream, map_w, map_x, p));
 }
 
-template <int DT>
+// tokens per tile of the few-row form, or 0 for pairs
+int few_row_tokens(const Product& q) {
+    if (q.a_mn) return 0;
+    const int key = fpt::tuning_linear_tokens();
+    return key >= 0 ? key : q.m <= 16 ? 16 : q.m <= 32 ? 32 : q.m <= 64 ? 64 : q.m <= 256 ? 128 : 0;
+}
+
+template <int DT, int ACT, bool SLOPE, bool A_MN, bool B_MN>
 int launch_product(const Product& q, LinearParams& p, const DeviceInfo& dev, cudaStream_t stream) {
     p.m = int(q.m);
     p.n = int(q.n);
     p.k_blocks = int((q.k + kBlockK - 1) / kBlockK);
-    const int key = fpt::tuning_linear_tokens();
-    int tokens = key >= 0 ? key : q.m <= 16 ? 16 : q.m <= 32 ? 32 : q.m <= 64 ? 64 : q.m <= 256 ? 128 : 0;
-    if (q.a_mn) tokens = 0;
-    if (tokens) {
+    const int tokens = few_row_tokens(q);
+    if constexpr (!A_MN) {
         // as many blocks as are resident together (two an SM), at least two K blocks each
-        const int64_t tiles = (q.m + tokens - 1) / tokens * ((q.n + 127) / 128);
+        const int64_t tiles = tokens ? (q.m + tokens - 1) / tokens * ((q.n + 127) / 128) : 1;
         int split = int(std::max<int64_t>(1, std::min<int64_t>(kMaxSplit, 2 * dev.sm_count / tiles)));
         if (fpt::tuning_linear_split() > 0) split = fpt::tuning_linear_split();
         split = std::max(1, std::min(split, p.k_blocks / 2));
-        auto by_weight = [&](auto t) {
-            constexpr int T = decltype(t)::value;
-            return q.b_mn ? launch_split<DT, T, true>(q, p, dev, split, stream) : launch_split<DT, T, false>(q, p, dev, split, stream);
-        };
-        if (tokens == 16) return by_weight(IC<16>{});
-        if (tokens == 32) return by_weight(IC<32>{});
-        if (tokens == 64) return by_weight(IC<64>{});
-        return by_weight(IC<128>{});
+        if (tokens == 16) return launch_split<DT, ACT, SLOPE, 16, B_MN>(q, p, dev, split, stream);
+        if (tokens == 32) return launch_split<DT, ACT, SLOPE, 32, B_MN>(q, p, dev, split, stream);
+        if (tokens == 64) return launch_split<DT, ACT, SLOPE, 64, B_MN>(q, p, dev, split, stream);
+        if (tokens == 128) return launch_split<DT, ACT, SLOPE, 128, B_MN>(q, p, dev, split, stream);
     }
-    if (q.a_mn) return q.b_mn ? launch_pair<DT, true, true>(q, p, dev, stream) : FPT_ERR_UNSUPPORTED_SHAPE;
-    return q.b_mn ? launch_pair<DT, false, true>(q, p, dev, stream) : launch_pair<DT, false, false>(q, p, dev, stream);
+    return launch_pair<DT, ACT, SLOPE, A_MN, B_MN>(q, p, dev, stream);
 }
 
 bool aligned16(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }
@@ -933,10 +980,18 @@ int check_sizes(int64_t rows, int64_t dim, int64_t out, int dtype) {
     return FPT_OK;
 }
 
+template <int ACT, bool SLOPE, bool A_MN, bool B_MN>
 int run_product(const Product& q, LinearParams& p, int dtype, cudaStream_t stream) {
     DeviceInfo dev;
     if (int rc = current_device_info(&dev)) return rc;
-    return dtype == FPT_BF16 ? launch_product<kBf16>(q, p, dev, stream) : launch_product<kFp16>(q, p, dev, stream);
+    return dtype == FPT_BF16 ? launch_product<kBf16, ACT, SLOPE, A_MN, B_MN>(q, p, dev, stream)
+                             : launch_product<kFp16, ACT, SLOPE, A_MN, B_MN>(q, p, dev, stream);
+}
+template <int ACT>
+int run_forward(const Product& q, LinearParams& p, int dtype, cudaStream_t stream) {
+    if constexpr (ACT != kNone)
+        if (p.slope) return run_product<ACT, true, false, false>(q, p, dtype, stream);
+    return run_product<ACT, false, false, false>(q, p, dtype, stream);
 }
 
 }  // namespace
@@ -954,10 +1009,8 @@ extern "C" int fpt_linear(void* out, void* slope, const void* x, const void* wei
         return FPT_ERR_BAD_ENUM;
     if (source != FPT_SRC_CURRENT && source != FPT_SRC_SOLLYA) return FPT_ERR_BAD_ENUM;
     LinearParams p{};
-    p.act.kind = function == FPT_FN_NONE ? kActNone : degree == 0 ? kActNative : kActProgram;
-    p.act.fn = function;
-    if (function == FPT_FN_NONE && degree != 0) return FPT_ERR_UNKNOWN_PROGRAM;
-    if (p.act.kind == kActProgram) {
+    if (function == FPT_FN_NONE && (degree != 0 || slope)) return FPT_ERR_UNKNOWN_PROGRAM;
+    if (degree != 0) {
         const ProgramRow* fwd = find_program(function, FPT_FWD, degree, dtype, source);
         const ProgramRow* bwd = find_program(function, FPT_BWD, degree, dtype, source);
         if (!fwd || (slope && !bwd)) return FPT_ERR_UNKNOWN_PROGRAM;
@@ -992,7 +1045,14 @@ extern "C" int fpt_linear(void* out, void* slope, const void* x, const void* wei
     p.vec_bias = reinterpret_cast<uintptr_t>(bias) % 16 == 0;
     p.status = static_cast<uint32_t*>(status);
     const Product q{x, weight, x_ld, w_ld, rows, out_features, dim, false, false};
-    return run_product(q, p, dtype, stream);
+    if (degree != 0) return run_forward<kProgram>(q, p, dtype, stream);
+    switch (function) {
+    case FPT_FN_SIGMOID: return run_forward<kSigmoid>(q, p, dtype, stream);
+    case FPT_FN_TANH: return run_forward<kTanh>(q, p, dtype, stream);
+    case FPT_FN_SWISH: return run_forward<kSwishAct>(q, p, dtype, stream);
+    case FPT_FN_GELU: return run_forward<kGelu>(q, p, dtype, stream);
+    default: return run_forward<kNone>(q, p, dtype, stream);
+    }
 }
 
 extern "C" int fpt_linear_grad_input(void* dx, const void* dz, const void* weight, int64_t rows, int64_t dim, int64_t out_features,
@@ -1008,7 +1068,7 @@ extern "C" int fpt_linear_grad_input(void* dx, const void* dz, const void* weigh
     p.vec_out = aligned16(dx, dx_ld);
     p.status = static_cast<uint32_t*>(status);
     const Product q{dz, weight, dz_ld, w_ld, rows, dim, out_features, false, true};
-    return run_product(q, p, dtype, stream);
+    return run_product<kNone, false, false, true>(q, p, dtype, stream);
 }
 
 extern "C" int fpt_linear_grad_weight(void* dw, const void* dz, const void* x, int64_t rows, int64_t dim, int64_t out_features,
@@ -1031,7 +1091,7 @@ extern "C" int fpt_linear_grad_weight(void* dw, const void* dz, const void* x, i
     p.vec_out = aligned16(dw, dw_ld);
     p.status = static_cast<uint32_t*>(status);
     const Product q{dz, x, dz_ld, x_ld, out_features, dim, rows, true, true};
-    return run_product(q, p, dtype, stream);
+    return run_product<kNone, false, true, true>(q, p, dtype, stream);
 }
 
 namespace {

@@ -361,7 +361,7 @@ __host__ __device__ constexpr uint32_t umma_idesc_bf16(uint32_t m, uint32_t n, u
 }  // namespace sm100
 
 // Host side: build a 4-D tiled tensor map over a bf16 tensor (dims innermost first, strides in bytes for dims 1..3),
-// box = {64, box_rows, 1, 1}, 128-byte swizzle, zero fill outside the tensor.  Returns an fpt status.
+// box = {64, box_rows, box_depth, 1}, 128-byte swizzle, zero fill outside the tensor.  Returns an fpt status.
 int make_tensor_map_bf16_4d(CUtensorMap* map, const void* base, const uint64_t dims[4], const uint64_t strides_bytes[3],
-                            uint32_t box_rows);
+                            uint32_t box_rows, uint32_t box_depth = 1);
 }  // namespace fpt

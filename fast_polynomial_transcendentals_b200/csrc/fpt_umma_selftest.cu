@@ -31,7 +31,7 @@ EncodeTiledFn encode_tiled_fn() {
 }  // namespace
 
 int make_tensor_map_bf16_4d(CUtensorMap* map, const void* base, const uint64_t dims[4], const uint64_t strides_bytes[3],
-                            uint32_t box_rows) {
+                            uint32_t box_rows, uint32_t box_depth) {
     EncodeTiledFn encode = encode_tiled_fn();
     if (!encode) return FPT_ERR_NO_DEVICE;
     if (reinterpret_cast<uintptr_t>(base) & 15u) return FPT_ERR_MISALIGNED;
@@ -39,7 +39,7 @@ int make_tensor_map_bf16_4d(CUtensorMap* map, const void* base, const uint64_t d
         if (strides_bytes[i] & 15u) return FPT_ERR_MISALIGNED;
     cuuint64_t gdim[4] = {dims[0], dims[1], dims[2], dims[3]};
     cuuint64_t gstride[3] = {strides_bytes[0], strides_bytes[1], strides_bytes[2]};
-    cuuint32_t box[4] = {64u, box_rows, 1u, 1u};
+    cuuint32_t box[4] = {64u, box_rows, box_depth, 1u};
     cuuint32_t estride[4] = {1u, 1u, 1u, 1u};
     const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), gdim, gstride, box, estride,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

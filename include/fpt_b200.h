@@ -406,7 +406,7 @@ int fpt_qk_norm_rope_bwd(void* dq, void* dk, void* dq_weight, void* dk_weight, c
  *      fp32 on the fp32 sums, one rounding at the end.  degree 3..6: the packed polynomial program of fpt_unary on the sums
  *      rounded to dtype (with a residual: its value plus the residual, rounded again).
  *      slope (fp16 [rows, out_features], whatever dtype) or null: act'(x W^T + b) for fpt_linear_grad_act; with a degree
- *      the derivative program of the same degree.
+ *      the derivative program of the same degree; null where there is no activation.
  *      status: one word the device can write and the host can read (mapped host memory serves; null: not reported): a
  *      bounded device-side wait that runs out stores 0x80000000 | where there, and the outputs of that call are invalid.
  *      It is not read when a call starts. */

@@ -51,7 +51,7 @@ def test_c_abi_checks_before_launch(fpt):
     assert call(function=3) == -5 and call(function=5) == -5 and call(source=2) == -5
     assert call(degree=3) == -4 and call(function=4, degree=9) == -4 and call(dtype=0, function=4, degree=5, source=1) == -4
     assert call(x=None) == -1 and call(out=None) == -1
-    assert call(x_ld=8) == -2 and call(w_ld=8) == -2 and call(out_ld=7) == -2 and call(r=p, res_ld=7) == -2 and call(slope=p, slope_ld=7) == -2
+    assert call(x_ld=8) == -2 and call(w_ld=8) == -2 and call(out_ld=7) == -2 and call(r=p, res_ld=7) == -2 and call(slope=p, slope_ld=7, function=4) == -2 and call(slope=p) == -4
     assert call(x=p + 8) == -3 and call(w_ld=20) == -3 and call(out=p + 1) == -3 and call(b=p + 2) == -3
     assert call(rows=0, x=None, out=None) == 0
 
