@@ -67,7 +67,7 @@ struct LinearParams {
     int ring;                       // stages of the ring
     uint32_t stage_bytes;           // their size, and the K blocks of 64 in one (pair form)
     int chunks;
-    bool a_whole, b_whole;          // one copy brings an operand's share of a stage (pair form)
+    bool a_whole, b_whole;          // one copy brings an operand's share of a stage
     int bias_dtype;
     bool vec_out, vec_res, vec_slope, vec_bias;
     bool staged;                    // out, residual and slope rows all start on 16-byte boundaries (pair form)
@@ -79,7 +79,10 @@ struct LinearParams {
 
 // Launched while the kernel before it drains (launch_early below): barriers and tensor memory are set up by then, and nothing of
 // global memory is touched before this.
-__device__ __forceinline__ void wait_for_inputs() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_inputs() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 
 __device__ __noinline__ void report(uint32_t* status, uint32_t where) {
     volatile uint32_t* s = status;
@@ -646,9 +649,13 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 if (turn > 0 && !wait(&sm.empty[s], (turn - 1u) & 1u, abort_flag, p.status, kWaitEmpty)) break;
                 uint8_t* stage = ring + s * kStageBytes;
                 mbar_arrive_expect_tx(&sm.full[s], kStageBytes);
-                if constexpr (W_MN) {
+                if (W_MN && p.b_whole) {
+                    tma_load_4d(stage, &map_w, &sm.full[s], 0, kb * kBlockK, output0 / 64, 0);
+                } else if (W_MN) {
                     tma_load_4d(stage, &map_w, &sm.full[s], output0, kb * kBlockK, 0, 0);
                     tma_load_4d(stage + kPanelBytes, &map_w, &sm.full[s], output0 + 64, kb * kBlockK, 0, 0);
+                } else if (p.b_whole) {
+                    tma_load_4d(stage, &map_w, &sm.full[s], 0, output0, kb, 0);
                 } else {
                     tma_load_4d(stage, &map_w, &sm.full[s], kb * kBlockK, output0, 0, 0);
                 }
@@ -842,9 +849,9 @@ int sliced_map(CUtensorMap* map, const void* base, int64_t rows, int64_t columns
     const uint64_t strides[3] = {uint64_t(ld) * 2, 128, uint64_t(ld) * 2 * uint64_t(rows)};
     return make_tensor_map_bf16_4d(map, base, dims, strides, uint32_t(box_rows), uint32_t(box_slices));
 }
-// one operand of the pair form, `size` of its rows per CTA and tile
+// one operand, `size` of its rows per CTA and tile
 // (an MN-major operand in slices starts its tiles on slices)
-int pair_map(CUtensorMap* map, bool* whole, const void* base, int64_t rows, int64_t k, int64_t ld, bool mn, int size, int chunks) {
+int tile_map(CUtensorMap* map, bool* whole, const void* base, int64_t rows, int64_t k, int64_t ld, bool mn, int size, int chunks) {
     *whole = mn ? rows % 64 == 0 && size % 64 == 0 : k % 64 == 0;
     if (mn) return *whole ? sliced_map(map, base, k, rows, ld, chunks * kBlockK, size > 64 ? 2 : 1) : operand_map(map, base, k, rows, ld, chunks * kBlockK);
     return *whole ? sliced_map(map, base, rows, k, ld, size, chunks) : operand_map(map, base, rows, k, ld, size);
@@ -907,8 +914,8 @@ int launch_pair(const Product& q, LinearParams& p, const DeviceInfo& dev, cudaSt
     p.columns = pair_columns(q, dev.sm_count / 2);
     p.chunks = kChunks;
     p.k_blocks = int((q.k + p.chunks * kBlockK - 1) / (p.chunks * kBlockK));
-    if (int rc = pair_map(&map_a, &p.a_whole, q.a, q.m, q.k, q.a_ld, A_MN, 128, p.chunks)) return rc;
-    if (int rc = pair_map(&map_b, &p.b_whole, q.b, q.n, q.k, q.b_ld, B_MN, p.columns / 2, p.chunks)) return rc;
+    if (int rc = tile_map(&map_a, &p.a_whole, q.a, q.m, q.k, q.a_ld, A_MN, 128, p.chunks)) return rc;
+    if (int rc = tile_map(&map_b, &p.b_whole, q.b, q.n, q.k, q.b_ld, B_MN, p.columns / 2, p.chunks)) return rc;
     p.m_tiles = int((q.m + 255) / 256);
     p.n_tiles = int((q.n + p.columns - 1) / p.columns);
     p.stage_bytes = share_bytes<A_MN>(128, p.chunks) + share_bytes<B_MN>(p.columns / 2, p.chunks);
@@ -924,27 +931,61 @@ int launch_pair(const Product& q, LinearParams& p, const DeviceInfo& dev, cudaSt
 template <int DT, int ACT, bool SLOPE, int TOKENS, bool W_MN>
 int launch_split(const Product& q, LinearParams& p, const DeviceInfo& dev, int split, cudaStream_t stream) {
     CUtensorMap map_w, map_x;
-    if (int rc = W_MN ? operand_map(&map_w, q.b, q.k, q.n, q.b_ld, kBlockK) : operand_map(&map_w, q.b, q.n, q.k, q.b_ld, 128)) return rc;
+    if (int rc = tile_map(&map_w, &p.b_whole, q.b, q.n, q.k, q.b_ld, W_MN, 128, 1)) return rc;
     if (int rc = operand_map(&map_x, q.a, q.m, q.k, q.a_ld, TOKENS)) return rc;
     p.m_tiles = int((q.m + TOKENS - 1) / TOKENS);
     p.n_tiles = int((q.n + 127) / 128);
     p.split = split;
     const int64_t blocks = int64_t(p.m_tiles) * p.n_tiles * split;
     if (blocks > 0x7fffffff) return FPT_ERR_BAD_SIZE;
-    // all the shared memory where every block has an SM to itself, else two blocks an SM
+    // all the shared memory where every block can have an SM to itself (clusters do not pack into every last one: 16 clusters
+    // of 8 or 48 of 3 took two rounds), else two blocks an SM
     const uint32_t stage = kTileBytes + TOKENS * 128;
-    const uint32_t budget = blocks <= dev.sm_count ? 216u * 1024u : 108u * 1024u;
+    const uint32_t budget = (split == 1 ? blocks <= dev.sm_count : split <= 4 && blocks <= dev.sm_count * 7 / 8) ? 216u * 1024u : 108u * 1024u;
     p.ring = int(std::min<uint32_t>(kMaxRing, budget / stage));
     const size_t smem = 1024 + kSplitRingOffset + std::max<size_t>(size_t(p.ring) * stage, size_t(TOKENS) * 512);
     return cuda_status(launch_early(linear_split_kernel<DT, ACT, SLOPE, TOKENS, W_MN>, unsigned(blocks), kSplitThreads, smem,
                                       split > 1 ? unsigned(split) : 0u, stream, map_w, map_x, p));
 }
 
-// tokens per tile of the few-row form, or 0 for pairs
-int few_row_tokens(const Product& q) {
-    if (q.a_mn) return 0;
-    const int key = fpt::tuning_linear_tokens();
-    return key >= 0 ? key : q.m <= 16 ? 16 : q.m <= 32 ? 32 : q.m <= 64 ? 64 : q.m <= 256 ? 128 : 0;
+// Which form, by the time it should take, in nanoseconds.  The terms were fitted to a sweep of both forms over six layers (512 x
+// 512 to 14336 x 4096, 1 to 1024 rows); the picks lie within some 5 % of the best measured.
+//   few rows   3000 to start and end, 28 per token of a tile (read-out), 300 for a cluster; the stream takes the longest of 210
+//              per K block and block on an SM, the weight at 6 TB/s and the tiles at 14 TB/s
+//   pairs      3600 + 9.5 per column to start, read out and end; 110 + 0.95 per column per K block and round
+// Clusters of five and seven are left out: seven blocks do not pack into a processing cluster of the chip (twice the time).
+struct Form {
+    int tokens, split;                 // tokens 0: pairs
+};
+Form choose_form(const Product& q, int k_blocks, int sm_count) {
+    const int64_t kb = k_blocks;
+    const int columns = pair_columns(q, sm_count / 2);
+    const int64_t pair_tiles = (q.m + 255) / 256 * ((q.n + columns - 1) / columns), rounds = (pair_tiles + sm_count / 2 - 1) / (sm_count / 2);
+    int64_t least = 3600 + 95 * columns / 10 + rounds * kb * (2200 + 19 * columns) / 20;
+    Form best{0, 1};
+    const int key = fpt::tuning_linear_tokens(), split_key = fpt::tuning_linear_split();
+    if (key > 0) least = INT64_MAX;
+    if (q.a_mn || key == 0) return best;
+    for (int tokens = 16; tokens <= 128; tokens *= 2) {
+        if (key > 0 && tokens != key) continue;
+        if (key < 0 && q.m > 8 * tokens) continue;
+        const int64_t tiles = (q.m + tokens - 1) / tokens * ((q.n + 127) / 128);
+        for (int split = 1; split <= kMaxSplit && (split == 1 || split <= kb / 2); ++split) {
+            if (split_key > 0 && split != std::max<int64_t>(1, std::min<int64_t>(split_key, kb / 2))) continue;
+            const int64_t blocks = tiles * split, per_sm = (blocks + sm_count - 1) / sm_count;
+            if (split_key <= 0 && (split == 5 || split == 7)) continue;
+            // one round of blocks, with room for the larger clusters to find their place
+            if (split > 1 && blocks > (split > 2 ? 256 * sm_count / 148 : 2 * sm_count) && split_key <= 0) break;
+            const int64_t issue = 210 * per_sm * ((kb + split - 1) / split);
+            const int64_t weight = q.n * q.k * 2 / 6000, traffic = tiles * kb * (16384 + 128 * tokens) / 14000;
+            const int64_t time = 3000 + 28 * tokens + (split > 1 ? 300 : 0) + std::max(issue, std::max(weight, traffic));
+            if (time < least) {
+                least = time;
+                best = Form{tokens, split};
+            }
+        }
+    }
+    return best;
 }
 
 template <int DT, int ACT, bool SLOPE, bool A_MN, bool B_MN>
@@ -952,17 +993,15 @@ int launch_product(const Product& q, LinearParams& p, const DeviceInfo& dev, cud
     p.m = int(q.m);
     p.n = int(q.n);
     p.k_blocks = int((q.k + kBlockK - 1) / kBlockK);
-    const int tokens = few_row_tokens(q);
     if constexpr (!A_MN) {
-        // as many blocks as are resident together (two an SM), at least two K blocks each
-        const int64_t tiles = tokens ? (q.m + tokens - 1) / tokens * ((q.n + 127) / 128) : 1;
-        int split = int(std::max<int64_t>(1, std::min<int64_t>(kMaxSplit, 2 * dev.sm_count / tiles)));
-        if (fpt::tuning_linear_split() > 0) split = fpt::tuning_linear_split();
-        split = std::max(1, std::min(split, p.k_blocks / 2));
-        if (tokens == 16) return launch_split<DT, ACT, SLOPE, 16, B_MN>(q, p, dev, split, stream);
-        if (tokens == 32) return launch_split<DT, ACT, SLOPE, 32, B_MN>(q, p, dev, split, stream);
-        if (tokens == 64) return launch_split<DT, ACT, SLOPE, 64, B_MN>(q, p, dev, split, stream);
-        if (tokens == 128) return launch_split<DT, ACT, SLOPE, 128, B_MN>(q, p, dev, split, stream);
+        const Form form = choose_form(q, p.k_blocks, dev.sm_count);
+        switch (form.tokens) {
+        case 16: return launch_split<DT, ACT, SLOPE, 16, B_MN>(q, p, dev, form.split, stream);
+        case 32: return launch_split<DT, ACT, SLOPE, 32, B_MN>(q, p, dev, form.split, stream);
+        case 64: return launch_split<DT, ACT, SLOPE, 64, B_MN>(q, p, dev, form.split, stream);
+        case 128: return launch_split<DT, ACT, SLOPE, 128, B_MN>(q, p, dev, form.split, stream);
+        default: break;
+        }
     }
     return launch_pair<DT, ACT, SLOPE, A_MN, B_MN>(q, p, dev, stream);
 }

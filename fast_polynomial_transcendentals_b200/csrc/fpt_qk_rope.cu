@@ -41,6 +41,12 @@ template <class T, bool NORM>
 constexpr int kFwdBlocks = sizeof(T) == 4 ? 2 : NORM ? 3 : 4;
 constexpr int kBwdBlocks = 2;
 
+// Launched while the kernel before it drains; nothing of global memory is touched before this.
+__device__ __forceinline__ void wait_for_inputs() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // n / d for n < 2^31 by a multiplication (Granlund and Montgomery, division by invariant integers): with l = ceil(log2 d)
 // and m = ceil(2^(31 + l) / d), floor(n m / 2^(31 + l)) is exact because n (m d - 2^(31 + l)) < 2^31 2^l.
 struct Divider {
@@ -457,6 +463,7 @@ __global__ void __launch_bounds__(kThreads, (kFwdBlocks<T, NORM>)) qk_rope_kerne
     const uint32_t lo = uint32_t(at.lo) * sizeof(T), hi = uint32_t(at.hi) * sizeof(T), out_bytes = uint32_t(a.dim) * sizeof(T);
     const float inv_dim = 1.0f / float(a.dim);
 
+    wait_for_inputs();
     float weight[2];                               // on their way to shared memory under the first loads of x
     if constexpr (NORM) {
         weight[0] = fetch_weight<C, HALVES>(a.side[0], a);
@@ -548,6 +555,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_norm_rope_bwd_kernel(
     const uint32_t heads = side.heads, step = kGroups / side.tile_tokens, group = threadIdx.x / G;
     const uint32_t my_slot = group / step, head = group % step, rounds = (heads + step - 1) / step;
     const bool one = side.tile_tokens == 1;
+    wait_for_inputs();
     // loads run ahead over the tiles: where they are
     uint32_t ahead_tile = block, ahead_round = 0, ahead_stage = 0, row = 0, row_g = 0;
     const char *x = nullptr, *grad = nullptr;
@@ -684,7 +692,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_norm_rope_bwd_kernel(
 __global__ void __launch_bounds__(256) weight_grad_kernel(const float* __restrict__ q_partial, const float* __restrict__ k_partial,
                                                           void* q_out, void* k_out, int q_blocks, int k_blocks, int dim, int dtype) {
     __shared__ float part[256];
-    asm volatile("griddepcontrol.wait;" ::: "memory");      // launched before the blocks it sums up have finished
+    wait_for_inputs();
     const float* partial = blockIdx.y ? k_partial : q_partial;
     void* out = blockIdx.y ? k_out : q_out;
     const int blocks = blockIdx.y ? k_blocks : q_blocks;
@@ -793,14 +801,24 @@ int prepare(QkRopeArgs& a, const void* q, const void* k, void* q_out, void* k_ou
     return FPT_OK;
 }
 
-template <class K>
-int launch(K kernel, unsigned grid, int smem, cudaStream_t stream, const QkRopeArgs& a) {
+// a launch that may begin while the kernel before it in the stream drains
+template <class... P, class... A>
+int launch(void (*kernel)(P...), dim3 grid, int smem, cudaStream_t stream, const A&... args) {
     if (smem > 32 * 1024) {            // with the static part, above what a kernel has unasked
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return int(e);
     }
-    kernel<<<grid, kThreads, smem, stream>>>(a);
-    return cuda_status(cudaGetLastError());
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = size_t(smem);
+    config.stream = stream;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&config, kernel, P(args)...));
 }
 
 // f(type, run, group, pairing) with compile-time arguments
@@ -904,6 +922,11 @@ extern "C" int fpt_qk_norm_rope_bwd(void* dq, void* dk, void* dq_weight, void* d
     const size_t item = dtype == FPT_FP32 ? 4 : 2;
     if (a.tokens) {
         if ((q_heads && (!dq_out || !dq_out_strides)) || (k_heads && (!dk_out || !dk_out_strides))) return FPT_ERR_NULL_POINTER;
+        for (int s = 0; s < 2; ++s) {
+            Side& d = a.side[s];
+            d.grad = s ? dk_out : dq_out;
+            if (d.heads && !rows_of(d.gs, d.grad, s ? dk_out_strides : dq_out_strides, batch, seq, d.heads, int64_t(item))) return FPT_ERR_MISALIGNED;
+        }
     }
     if (weights && reinterpret_cast<uintptr_t>(workspace) % 4) return FPT_ERR_MISALIGNED;
     DeviceInfo dev;
@@ -922,9 +945,6 @@ extern "C" int fpt_qk_norm_rope_bwd(void* dq, void* dk, void* dq_weight, void* d
         for (int s = 0; s < 2; ++s) {
             Side& d = a.side[s];
             if (!d.heads) continue;
-            const int64_t* st = s ? dk_out_strides : dq_out_strides;
-            d.grad = s ? dk_out : dq_out;
-            if (!rows_of(d.gs, d.grad, st, batch, seq, d.heads, int64_t(item))) return FPT_ERR_MISALIGNED;
             d.tile_tokens = tile_tokens(groups, d.heads, uint32_t(pairs), 8, kBwdTrig);
             // no more tokens a tile than keep every block busy
             while (d.tile_tokens > 1 && a.tokens / d.tile_tokens < blocks[s]) d.tile_tokens /= 2;
@@ -944,18 +964,9 @@ extern "C" int fpt_qk_norm_rope_bwd(void* dq, void* dk, void* dq_weight, void* d
         if (rc) return rc;
     }
     if (weights) {                     // without tokens: zeros
-        cudaLaunchConfig_t config{};
-        config.gridDim = dim3(unsigned(head_dim / 8), 2);
-        config.blockDim = dim3(256);
-        config.stream = stream;
-        cudaLaunchAttribute attribute{};
-        attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attribute.val.programmaticStreamSerializationAllowed = 1;
-        config.attrs = &attribute;
-        config.numAttrs = a.tokens ? 1 : 0;
         const float* k_partial = partial ? partial + int64_t(blocks[0]) * head_dim : nullptr;
-        return cuda_status(cudaLaunchKernelEx(&config, weight_grad_kernel, static_cast<const float*>(partial), k_partial, dq_weight, dk_weight,
-                                              int(blocks[0]), int(blocks[1]), int(head_dim), weight_dtype));
+        return launch(weight_grad_kernel, dim3(unsigned(head_dim / 8), 2), 0, stream, partial, k_partial, dq_weight, dk_weight,
+                      int(blocks[0]), int(blocks[1]), int(head_dim), weight_dtype);
     }
     return FPT_OK;
 }

@@ -12,11 +12,15 @@
 // pass of a small call is then a few microseconds of host time.  They are not themselves differentiable and say so.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 #include <torch/library.h>
 
 #include <cmath>
+#include <memory>
+#include <mutex>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -209,42 +213,38 @@ std::tuple<Tensor, Tensor> call_qk_rope(const Tensor& q, const Tensor& k, const 
     return op.call(q, k, q_weight, k_weight, increments, positions, sections, order, pairing, norm, eps, inverse);
 }
 
-struct QkRopeFunction : torch::autograd::Function<QkRopeFunction> {
-    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k,
-                                                  const OptTensor& q_weight, const OptTensor& k_weight, const Tensor& increments,
-                                                  const OptTensor& positions, std::vector<int64_t> sections, int64_t order,
-                                                  int64_t pairing, bool norm, double eps, bool inverse) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        auto out = call_qk_rope(q, k, q_weight, k_weight, increments, positions, sections, order, pairing, norm, eps, inverse);
-        // the rotation alone needs neither q nor k again
-        ctx->save_for_backward({norm ? q : Tensor(), norm ? k : Tensor(), q_weight.value_or(Tensor()), k_weight.value_or(Tensor()),
-                                increments, positions.value_or(Tensor())});
-        ctx->saved_data["sections"] = sections;
-        ctx->saved_data["order"] = order;
-        ctx->saved_data["pairing"] = pairing;
-        ctx->saved_data["norm"] = norm;
-        ctx->saved_data["eps"] = eps;
-        ctx->saved_data["inverse"] = inverse;
-        ctx->saved_data["dq_weight"] = q_weight.has_value() && q_weight->requires_grad();
-        ctx->saved_data["dk_weight"] = k_weight.has_value() && k_weight->requires_grad();
-        return {std::get<0>(out), std::get<1>(out)};
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+
+// a node like the generated ones of the library itself: a third of the host time of the generic custom function
+struct QkRopeBackward : torch::autograd::Node {
+    SavedVariable q, k, q_weight, k_weight, increments, positions;
+    std::vector<int64_t> sections;
+    int64_t order = 0, pairing = 0;
+    bool norm = false, inverse = false, has_q_weight = false, has_k_weight = false, has_positions = false;
+    double eps = 0;
+
+    std::string name() const override { return "QkRopeBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable* v : {&q, &k, &q_weight, &k_weight, &increments, &positions}) v->reset_data();
     }
-    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
         no_second_gradient("qk_rope");
-        const auto saved = ctx->get_saved_variables();
-        const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
-        const auto sections = ctx->saved_data["sections"].toIntVector();
-        const int64_t order = ctx->saved_data["order"].toInt(), pairing = ctx->saved_data["pairing"].toInt();
-        torch::autograd::variable_list out(12);
-        if (!ctx->saved_data["norm"].toBool()) {
-            std::tie(out[0], out[1]) = call_qk_rope(grads[0], grads[1], {}, {}, saved[4], opt(saved[5]), sections, order, pairing,
-                                                    false, 0.0, !ctx->saved_data["inverse"].toBool());
+        variable_list out(4);
+        for (int i = 0; i < 2; ++i)
+            if (!grads[i].defined()) grads[i] = input_metadata(i).zeros_like();
+        const OptTensor pos = has_positions ? OptTensor(positions.unpack()) : OptTensor();
+        const Tensor inc = increments.unpack();
+        if (!norm) {                    // the rotation alone needs neither q nor k again
+            std::tie(out[0], out[1]) = call_qk_rope(grads[0], grads[1], {}, {}, inc, pos, sections, order, pairing, false, 0.0, !inverse);
             return out;
         }
         static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::qk_norm_rope_bwd", "").typed<decltype(qk_norm_rope_bwd)>();
-        const bool dqw = ctx->saved_data["dq_weight"].toBool(), dkw = ctx->saved_data["dk_weight"].toBool();
-        auto d = op.call(grads[0], grads[1], saved[0], saved[1], opt(saved[2]), opt(saved[3]), saved[4], opt(saved[5]), sections, order,
-                         pairing, ctx->saved_data["eps"].toDouble(), dqw, dkw);
+        const bool dqw = has_q_weight && task_should_compute_output(2), dkw = has_k_weight && task_should_compute_output(3);
+        auto d = op.call(grads[0], grads[1], q.unpack(), k.unpack(), has_q_weight ? OptTensor(q_weight.unpack()) : OptTensor(),
+                         has_k_weight ? OptTensor(k_weight.unpack()) : OptTensor(), inc, pos, sections, order, pairing, eps, dqw, dkw);
         out[0] = std::get<0>(d);
         out[1] = std::get<1>(d);
         if (dqw) out[2] = std::get<2>(d);
@@ -256,14 +256,35 @@ struct QkRopeFunction : torch::autograd::Function<QkRopeFunction> {
 std::tuple<Tensor, Tensor> qk_rope_autograd(const Tensor& q, const Tensor& k, const OptTensor& q_weight, const OptTensor& k_weight,
                                             const Tensor& increments, const OptTensor& positions, at::IntArrayRef sections,
                                             int64_t order, int64_t pairing, bool norm, double eps, bool inverse) {
-    const bool wanted = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || (q_weight && q_weight->requires_grad()) ||
-                                                       (k_weight && k_weight->requires_grad()));
-    if (!wanted) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        return call_qk_rope(q, k, q_weight, k_weight, increments, positions, sections, order, pairing, norm, eps, inverse);
+    const Tensor qw = q_weight.value_or(Tensor()), kw = k_weight.value_or(Tensor());
+    std::shared_ptr<QkRopeBackward> node;
+    if (torch::autograd::compute_requires_grad(q, k, qw, kw)) {
+        node = std::shared_ptr<QkRopeBackward>(new QkRopeBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(q, k, qw, kw));
+        if (norm) {
+            node->q = SavedVariable(q, false);
+            node->k = SavedVariable(k, false);
+        }
+        node->has_q_weight = qw.defined();
+        node->has_k_weight = kw.defined();
+        if (qw.defined()) node->q_weight = SavedVariable(qw, false);
+        if (kw.defined()) node->k_weight = SavedVariable(kw, false);
+        node->increments = SavedVariable(increments, false);
+        node->has_positions = positions.has_value();
+        if (positions) node->positions = SavedVariable(*positions, false);
+        node->sections = sections.vec();
+        node->order = order, node->pairing = pairing, node->norm = norm, node->eps = eps, node->inverse = inverse;
     }
-    auto out = QkRopeFunction::apply(q, k, q_weight, k_weight, increments, positions, sections.vec(), order, pairing, norm, eps, inverse);
-    return {out[0], out[1]};
+    std::tuple<Tensor, Tensor> out;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        out = call_qk_rope(q, k, q_weight, k_weight, increments, positions, sections, order, pairing, norm, eps, inverse);
+    }
+    if (node) {
+        torch::autograd::set_history(std::get<0>(out), node);
+        torch::autograd::set_history(std::get<1>(out), node);
+    }
+    return out;
 }
 
 // ---- fpt_linear -----------------------------------------------------------------------------------------------------
@@ -436,57 +457,65 @@ Tensor call_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias,
     return op.call(x, weight, bias, residual, function, degree, source);
 }
 
-struct LinearFunction : torch::autograd::Function<LinearFunction> {
-    static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias,
-                          const OptTensor& residual, int64_t function, int64_t degree, int64_t source) {
-        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::linear_act_slope", "").typed<decltype(linear_act_slope)>();
-        at::AutoDispatchBelowADInplaceOrView below;
-        const bool want_x = x.requires_grad(), want_w = weight.requires_grad(), want_b = bias && bias->requires_grad();
-        Tensor out, slope;
-        if (function == FPT_FN_NONE || !(want_x || want_w || want_b)) {          // the slope is 1, or nobody asks for it
-            out = call_linear(x, weight, bias, residual, function, degree, source);
-            slope = at::empty({0, (weight.size(0) + 7) / 8 * 8}, x.options().dtype(at::kHalf));
-        } else {
-            std::tie(out, slope) = op.call(x, weight, bias, residual, function, degree, source);
-        }
-        ctx->save_for_backward({want_w ? x : Tensor(), want_x ? weight : Tensor(), slope});
-        ctx->saved_data["shape"] = x.sizes().vec();
-        ctx->saved_data["out"] = weight.size(0);
-        ctx->saved_data["bias_dtype"] = int64_t(bias ? dtype_id(bias->scalar_type()) : FPT_FP32);
-        ctx->saved_data["x"] = want_x;
-        ctx->saved_data["weight"] = want_w;
-        ctx->saved_data["bias"] = want_b;
-        ctx->saved_data["residual"] = residual && residual->requires_grad();
-        return out;
+struct LinearBackward : torch::autograd::Node {
+    SavedVariable x, weight, slope;
+    std::vector<int64_t> shape;         // of x
+    int64_t out = 0, bias_dtype = 0;
+    bool has_bias = false;
+
+    std::string name() const override { return "LinearActBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable* v : {&x, &weight, &slope}) v->reset_data();
     }
-    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
         no_second_gradient("linear_act");
-        const auto saved = ctx->get_saved_variables();
-        const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
-        const bool want_x = ctx->saved_data["x"].toBool(), want_w = ctx->saved_data["weight"].toBool(), want_b = ctx->saved_data["bias"].toBool();
-        torch::autograd::variable_list out(7);
+        variable_list result(4);
+        if (!grads[0].defined()) return result;
+        const bool want_x = task_should_compute_output(0), want_w = task_should_compute_output(1), want_b = has_bias && task_should_compute_output(2);
         if (want_x || want_w || want_b) {
             static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::linear_act_bwd", "").typed<decltype(linear_act_bwd)>();
-            auto d = op.call(grads[0], saved[2], opt(saved[0]), opt(saved[1]), ctx->saved_data["shape"].toIntVector(), ctx->saved_data["out"].toInt(),
-                             ctx->saved_data["bias_dtype"].toInt(), want_x, want_w, want_b);
-            if (want_x) out[0] = std::get<0>(d);
-            if (want_w) out[1] = std::get<1>(d);
-            if (want_b) out[2] = std::get<2>(d);
+            auto d = op.call(grads[0], slope.unpack(), want_w ? OptTensor(x.unpack()) : OptTensor(), want_x ? OptTensor(weight.unpack()) : OptTensor(),
+                             shape, out, bias_dtype, want_x, want_w, want_b);
+            if (want_x) result[0] = std::get<0>(d);
+            if (want_w) result[1] = std::get<1>(d);
+            if (want_b) result[2] = std::get<2>(d);
         }
-        if (ctx->saved_data["residual"].toBool()) out[3] = grads[0];
-        return out;
+        if (task_should_compute_output(3)) result[3] = grads[0];
+        return result;
     }
 };
 
 Tensor linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int64_t function,
                        int64_t degree, int64_t source) {
-    const bool wanted = at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()) ||
-                                                       (residual && residual->requires_grad()));
-    if (!wanted) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        return call_linear(x, weight, bias, residual, function, degree, source);
+    static const auto with_slope = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::linear_act_slope", "").typed<decltype(linear_act_slope)>();
+    const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+    std::shared_ptr<LinearBackward> node;
+    bool keep_slope = false;            // no activation: the slope is 1; only the residual wants a gradient: nobody asks for it
+    if (torch::autograd::compute_requires_grad(x, weight, b, r)) {
+        node = std::shared_ptr<LinearBackward>(new LinearBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x, weight, b, r));
+        if (weight.requires_grad()) node->x = SavedVariable(x, false);
+        if (x.requires_grad()) node->weight = SavedVariable(weight, false);
+        node->shape = x.sizes().vec();
+        node->out = weight.dim() ? weight.size(0) : 0;
+        node->has_bias = b.defined();
+        node->bias_dtype = b.defined() ? dtype_id(b.scalar_type()) : FPT_FP32;
+        keep_slope = function != FPT_FN_NONE && (x.requires_grad() || weight.requires_grad() || (b.defined() && b.requires_grad()));
     }
-    return LinearFunction::apply(x, weight, bias, residual, function, degree, source);
+    Tensor out, slope;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        if (keep_slope) std::tie(out, slope) = with_slope.call(x, weight, bias, residual, function, degree, source);
+        else out = call_linear(x, weight, bias, residual, function, degree, source);
+        if (node && !keep_slope) slope = at::empty({0, 8}, x.options().dtype(at::kHalf));
+    }
+    if (node) {
+        node->slope = SavedVariable(slope, false);
+        torch::autograd::set_history(out, node);
+    }
+    return out;
 }
 
 // the eager doors: off the GPU the checks run here, where no kernel would be found
