@@ -17,6 +17,7 @@ import torch
 from torch import nn
 
 from ..gate_up import gate_up_swiglu, gate_up_swiglu_recompute, grouped_linear
+from ..linear import linear_act
 from .activations import (resolve_mlp_activation_impl, resolve_mlp_activation_mul_impl,
                           resolve_mlp_activation_packed_impl)
 
@@ -231,6 +232,61 @@ def patch_grouped_experts(model: nn.Module, *, variant: str = "polynomial", degr
     return patched
 
 
+_MLP_PAIRS = (("fc1", "fc2"), ("up_proj", "down_proj"), ("c_fc", "c_proj"), ("dense_h_to_4h", "dense_4h_to_h"))
+
+
+def _epilogue_activation(fn: Any) -> str | None:
+    """'gelu' or 'silu' where `fn` is the erf GELU or SiLU; the tanh approximation of GELU is another function."""
+    if isinstance(fn, nn.GELU):
+        return "gelu" if fn.approximate == "none" else None
+    if isinstance(fn, nn.SiLU) or fn is torch.nn.functional.silu:
+        return "silu"
+    if fn is torch.nn.functional.gelu:
+        return "gelu"
+    return {"geluactivation": "gelu", "siluactivation": "silu"}.get(type(fn).__name__.lower())
+
+
+def patch_mlp_epilogues(model: nn.Module, *, variant: str = "native", degree: int | None = None, coeff_source: str = "current",
+                        skipped: list[tuple[str, str]] | None = None) -> int:
+    """down(act(up(x))) as two kernels, bias and activation in the first one's epilogue and the bias in the second's
+    (`linear.linear_act`), forward and backward; weights untouched, `restore` undoes it.
+
+    A module qualifies by structure: two `nn.Linear` under the usual names (`fc1 / fc2`, `up_proj / down_proj` without a gate,
+    ...), an erf GELU or SiLU in an activation slot, and nothing else that could act in between (dropout only where its
+    probability is zero); others with the two projections are left alone and reported through `skipped`.  variant "native"
+    evaluates the activation in fp32, "polynomial" runs the packed program (degree 5 for GELU, 3 for SiLU by default).
+    Inputs that are not float16 or bfloat16 on the GPU, or whose width is no multiple of 8, take the module's own forward."""
+    patched = 0
+    for name, module in model.named_modules():
+        pair = next((p for p in _MLP_PAIRS if all(isinstance(getattr(module, n, None), nn.Linear) for n in p)), None)
+        if pair is None or _projection_names(module) is not None:
+            continue
+        slot = next((a for a in _ACTIVATION_SLOTS if getattr(module, a, None) is not None), None)
+        activation = _epilogue_activation(getattr(module, slot)) if slot else None
+        others = [n for n, m in module.named_children() if n not in (*pair, slot)
+                  and not isinstance(m, nn.Identity) and not (isinstance(m, nn.Dropout) and m.p == 0)]
+        if activation is None or others:
+            if skipped is not None:
+                skipped.append((name, f"also holds {', '.join(others)}" if others else
+                                f"{slot}={type(getattr(module, slot)).__name__}" if slot else "no activation slot"))
+            continue
+        chosen = 0 if variant == "native" else degree if degree is not None else {"gelu": 5, "silu": 3}[activation]
+
+        def forward(self, x, *args, _up=pair[0], _down=pair[1], _act=activation, _degree=chosen, **kwargs):
+            up, down = getattr(self, _up), getattr(self, _down)
+            if not (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and up.weight.dtype == down.weight.dtype == x.dtype
+                    and up.weight.shape[1] % 8 == 0 and down.weight.shape[1] % 8 == 0) or torch.is_autocast_enabled("cuda"):
+                return self.__dict__[_ORIGINAL](x, *args, **kwargs)
+            hidden = linear_act(x, up.weight, up.bias, activation=_act, degree=_degree, coeff_source=coeff_source)
+            return linear_act(hidden, down.weight, down.bias)
+
+        if _ORIGINAL not in module.__dict__:
+            module.__dict__[_ORIGINAL] = module.forward
+        module.forward = MethodType(forward, module)
+        patched += 1
+    return patched
+
+
 class FunctionActivation(nn.Module):
     """An activation function in a slot that used to hold a module."""
 
@@ -262,7 +318,7 @@ def patch_activation_slots(model: nn.Module, *, kind: str = "silu", degree: int 
 
 
 def restore(model: nn.Module) -> int:
-    """Undo `patch_dense_swiglu`, `patch_grouped_experts` and `patch_activation_slots`."""
+    """Undo `patch_dense_swiglu`, `patch_grouped_experts`, `patch_mlp_epilogues` and `patch_activation_slots`."""
     restored = 0
     for module in model.modules():
         if hasattr(module, _ORIGINAL):
@@ -281,4 +337,4 @@ def restore(model: nn.Module) -> int:
 
 __all__ = ["FunctionActivation", "FusedGateUpFeedForward", "dense_swiglu_modules", "fuse_gate_up_projections",
            "gated_mlp_activation",
-           "patch_activation_slots", "patch_dense_swiglu", "patch_grouped_experts", "restore", "run_grouped_experts"]
+           "patch_activation_slots", "patch_dense_swiglu", "patch_grouped_experts", "patch_mlp_epilogues", "restore", "run_grouped_experts"]

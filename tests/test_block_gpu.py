@@ -1,0 +1,214 @@
+"""GPU: the operators around the attention in a run, as a transformer block uses them: projection with bias, norm of queries
+and keys with the rotation (one axis, or three), the attention kernel, projection onto the residual stream, GELU
+feed-forward onto the residual stream; forward, gradients, a captured step, and the feed-forward through the adapter."""
+import math
+
+import pytest
+import torch
+from torch import nn
+
+from fast_polynomial_transcendentals_b200 import qk_rope
+from fast_polynomial_transcendentals_b200.linear import check_linear_status, linear_act
+from fast_polynomial_transcendentals_b200.sfu_repro import adapters, fa4
+from fast_polynomial_transcendentals_b200.sfu_repro.rope import rope_phase_increments
+
+pytestmark = pytest.mark.gpu
+B, S, HQ, HK, D, HIDDEN = 2, 200, 4, 2, 128, 1000
+DIM = HQ * D
+BF = torch.bfloat16
+
+
+def weights(device, seed=0):
+    g = torch.Generator(device=device)
+    g.manual_seed(seed)
+    rand = lambda *s, scale=1.0: (torch.randn(*s, device=device, generator=g) * scale).to(BF)
+    return dict(qkv=rand((HQ + 2 * HK) * D, DIM, scale=DIM ** -0.5), qkv_bias=rand((HQ + 2 * HK) * D, scale=0.1),
+                q_norm=1 + rand(D, scale=0.1), k_norm=1 + rand(D, scale=0.1), out=rand(DIM, DIM, scale=DIM ** -0.5),
+                up=rand(HIDDEN, DIM, scale=DIM ** -0.5), up_bias=rand(HIDDEN, scale=0.1), down=rand(DIM, HIDDEN, scale=HIDDEN ** -0.5),
+                down_bias=rand(DIM, scale=0.1)), rand(B, S, DIM)
+
+
+def attention(q, k, v):
+    config = fa4.resolve_fa4_config(fa4.FA4Config(mode="softmax"), sequence_length=S)
+    return fa4._fa4(q, k, v, softmax_scale=None, causal=True, config=config)
+
+
+def split_heads(qkv):
+    return (qkv[..., :HQ * D].unflatten(-1, (HQ, D)), qkv[..., HQ * D:(HQ + HK) * D].unflatten(-1, (HK, D)),
+            qkv[..., (HQ + HK) * D:].unflatten(-1, (HK, D)))
+
+
+def block(x, w, inc, positions, sections):
+    q, k, v = split_heads(linear_act(x, w["qkv"], w["qkv_bias"]))
+    if sections is None:
+        q, k = qk_rope.qk_norm_rope(q, k, w["q_norm"], w["k_norm"], inc, positions=positions, pairing="halves")
+    else:
+        q, k = qk_rope.rope_axes(q, k, inc, positions, sections, pairing="halves")
+    x = linear_act(attention(q, k, v.contiguous()).flatten(2), w["out"], None, x)
+    return linear_act(linear_act(x, w["up"], w["up_bias"], activation="gelu"), w["down"], w["down_bias"], x)
+
+
+class RoundGrad(torch.autograd.Function):
+    """bf16 value, bf16 gradient: where an operator of the run hands on a tensor"""
+
+    @staticmethod
+    def forward(ctx, x):
+        return x.to(BF).float()
+
+    @staticmethod
+    def backward(ctx, g):
+        return g.to(BF).float()
+
+
+def plain_block(x, w, inc, positions, sections):
+    """The same in fp32 with roundings to bf16 at the operators' borders, around the same attention kernel."""
+    f = {n: t.float() for n, t in w.items()}
+    rnd = RoundGrad.apply
+    xf = x.float()
+    q, k, v = split_heads(rnd(xf @ f["qkv"].T + f["qkv_bias"]))
+    if sections is None:
+        position = positions[..., None].double()
+        q, k = (t * torch.rsqrt(t.square().mean(-1, keepdim=True) + 1e-6) * f[n] for t, n in ((q, "q_norm"), (k, "k_norm")))
+    else:
+        position = torch.stack([positions[a] for a, n in enumerate(sections) for _ in range(n)], dim=-1).double()
+    angle = (position * inc.double() * (2 * math.pi / 2 ** 32))[:, :, None]
+    c, s = angle.cos().float(), angle.sin().float()
+    turn = lambda t: rnd(torch.cat((t[..., :D // 2] * c - t[..., D // 2:] * s, t[..., D // 2:] * c + t[..., :D // 2] * s), dim=-1))
+    xf = rnd(attention(turn(q).to(BF), turn(k).to(BF), v.to(BF)).float().flatten(2) @ f["out"].T + xf)
+    hidden = rnd(torch.nn.functional.gelu(xf @ f["up"].T + f["up_bias"]))
+    return rnd(hidden @ f["down"].T + f["down_bias"] + xf)
+
+
+def case(cuda, axes):
+    w, x = weights(cuda)
+    inc = rope_phase_increments(D, 10000.0, cuda)
+    if axes:
+        return w, x, inc, torch.randint(0, 60, (3, B, S), device=cuda), [16, 24, 24]
+    return w, x, inc, torch.arange(S, device=cuda).expand(B, S) + torch.tensor([[0], [5000]], device=cuda), None
+
+
+@pytest.mark.parametrize("axes", [False, True])
+def test_a_block_and_its_gradients(cuda, axes):
+    """Both runs round at the same places, so values differ where a rounding falls the other way (one step, 2^-8 of the value,
+    carried on through up to six operators: root mean square below 2^-8); in the gradients the operators also round dz before
+    its products (2^-8 at most, 2^-9.3 root mean square, at three layers): below 2^-7."""
+    w, x, inc, positions, sections = case(cuda, axes)
+    leaves = {n: t.detach().requires_grad_() for n, t in w.items() if not (axes and n.endswith("_norm"))}
+    xs = x.detach().requires_grad_()
+    names = ["x", *leaves]
+    grad = torch.randn_like(x)
+    results = []
+    for f in (block, plain_block):
+        y = f(xs, {**w, **leaves}, inc, positions, sections)
+        results.append((y.detach().float(), torch.autograd.grad(y, [xs, *leaves.values()], grad.to(y.dtype))))
+    relative = lambda a, b: ((a.float() - b.float()).norm() / b.float().norm()).item()
+    assert relative(results[0][0], results[1][0]) < 2.0 ** -8
+    for n, a, b in zip(names, results[0][1], results[1][1]):
+        assert relative(a, b) < 2.0 ** -7, (n, relative(a, b))
+    fa4.check_attention_status()
+    check_linear_status()
+
+
+def test_a_captured_step(cuda):
+    """Forward and backward of the run in one graph, replayed with new inputs; the attention adds its dQ in no fixed order, so
+    only what does not pass through it is compared bit for bit."""
+    w, x, inc, positions, sections = case(cuda, False)
+    leaves = {n: t.detach().requires_grad_() for n, t in w.items()}
+    grad = torch.randn_like(x)
+
+    def step():
+        y = block(x, leaves, inc, positions, sections)
+        return y, *torch.autograd.grad(y, [leaves["up"], leaves["down"], leaves["up_bias"]], grad)
+
+    stream = torch.cuda.Stream(cuda)
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = step()
+    for _ in range(2):
+        x.copy_(torch.randn_like(x))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))
+    fa4.check_attention_status()
+    check_linear_status()
+
+
+def test_one_token_at_a_time_equals_the_prompt(cuda):
+    """Serving: the projections, norms and rotations of single tokens at their positions give what the whole prompt gives, up
+    to the order of the fp32 sums (another tile form), one step of bf16."""
+    w, x, inc, positions, _ = case(cuda, False)
+    whole = split_heads(linear_act(x, w["qkv"], w["qkv_bias"]))
+    q, k = qk_rope.qk_norm_rope(*whole[:2], w["q_norm"], w["k_norm"], inc, positions=positions, pairing="halves")
+    for t in (0, 1, 77, S - 1):
+        one = split_heads(linear_act(x[:, t:t + 1], w["qkv"], w["qkv_bias"]))
+        q1, k1 = qk_rope.qk_norm_rope(*one[:2], w["q_norm"], w["k_norm"], inc, positions=positions[:, t:t + 1], pairing="halves")
+        for a, b in ((q1, q[:, t:t + 1]), (k1, k[:, t:t + 1])):
+            # one step (2^-7 of the largest of a pair) of the projection, another of the result
+            assert (a.float() - b.float()).abs().max() <= 2 * 2.0 ** -7 * float(b.float().abs().max())
+            assert ((a.float() - b.float()).norm() / b.float().norm()).item() < 2.0 ** -9
+
+
+class Mlp(nn.Module):
+    def __init__(self, act):
+        super().__init__()
+        self.fc1, self.fc2, self.activation_fn = nn.Linear(256, 600), nn.Linear(600, 256), act
+
+    def forward(self, x):
+        return self.fc2(self.activation_fn(self.fc1(x)))
+
+
+@pytest.mark.parametrize("act", [nn.GELU(), nn.SiLU()], ids=["gelu", "silu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_adapter_runs_the_feed_forward(cuda, act, dtype):
+    """Against the same module in fp32: the patched one rounds the hidden values, dz and the results (four roundings of at
+    most eps / 2)."""
+    torch.manual_seed(1)
+    model = Mlp(act).to(cuda, dtype)
+    x, grad = torch.randn(70, 256, device=cuda).to(dtype).requires_grad_(), torch.randn(70, 256, device=cuda).to(dtype)
+    exact = Mlp(act).to(cuda)
+    exact.load_state_dict({n: t.float() for n, t in model.state_dict().items()})
+    xf = x.detach().float().requires_grad_()
+    want_y = exact(xf)
+    want = torch.autograd.grad(want_y, [xf, *exact.parameters()], grad.float())
+    assert adapters.patch_mlp_epilogues(model) == 1
+    y = model(x)
+    got = torch.autograd.grad(y, [x, *model.parameters()], grad)
+    for a, b in zip((y, *got), (want_y, *want)):
+        assert ((a.float() - b).norm() / b.norm()).item() < 4 * torch.finfo(dtype).eps / 2
+    poly = Mlp(act).to(cuda, dtype)
+    poly.load_state_dict(model.state_dict())
+    assert adapters.patch_mlp_epilogues(poly, variant="polynomial") == 1
+    assert ((poly(x).float() - want_y).norm() / want_y.norm()).item() < 0.05         # the programs' own error
+    assert adapters.restore(model) == 1
+    torch.testing.assert_close(model(x).float(), y.float(), rtol=0, atol=8 * torch.finfo(dtype).eps)
+    check_linear_status()
+
+
+def test_offsets_past_31_bits(cuda):
+    """Results of more than 2^31 elements, rows checked at both ends and in between.  One rounding to bf16 (eps / 2 = 2^-8 of
+    the value: eight significant bits) and fp32 sums of 64 terms of size 64 / 8 in all (18 u S, S < 100: below 3e-4)."""
+    rows, out = 66000, 33000
+    x, w = torch.randn(rows, 64, device=cuda).to(BF), torch.randn(out, 64, device=cuda).to(BF)
+    y = linear_act(x, w, activation="silu")
+    for i in (0, 1, 32767, 65535, 65536, rows - 1):
+        z = x[i].double() @ w.double().T
+        want = z * torch.sigmoid(z)
+        assert ((y[i].double() - want).abs() <= 2.0 ** -8 * want.abs() + 3e-4).all(), i
+    del y
+    seq = 270000                                       # 2 x 270000 x 32 x 128 > 2^31, and a batch entry beyond 4 GB of rows
+    wide = torch.empty(2, seq, 34 * 128 * 2, dtype=BF, device=cuda)
+    q = wide[..., :32 * 128].unflatten(-1, (32, 128))
+    k = wide[..., 32 * 128:34 * 128].unflatten(-1, (2, 128))
+    picks = [(0, 0), (0, 1), (0, 246723), (0, seq - 1), (1, 0), (1, 123456), (1, seq - 1)]
+    for b, s in picks:
+        wide[b, s] = torch.randn(wide.shape[-1], device=cuda).to(BF)
+    inc = rope_phase_increments(128, device=cuda)
+    got = qk_rope.rope_axes(q, k, inc, torch.arange(seq, device=cuda)[None], [64], pairing="halves")
+    for b, s in picks:
+        one = qk_rope.rope_axes(q[b:b + 1, s:s + 1].contiguous(), k[b:b + 1, s:s + 1].contiguous(), inc,
+                                torch.tensor([[s]], device=cuda), [64], pairing="halves")
+        assert torch.equal(got[0][b, s], one[0][0, 0]) and torch.equal(got[1][b, s], one[1][0, 0]), (b, s)

@@ -1,0 +1,45 @@
+"""CPU: which feed-forward modules the epilogue adapter takes, and that what it takes behaves as before off the GPU."""
+import torch
+from torch import nn
+
+from fast_polynomial_transcendentals_b200.sfu_repro import adapters
+
+
+class Mlp(nn.Module):
+    def __init__(self, act=None, dropout=None, names=("fc1", "fc2")):
+        super().__init__()
+        setattr(self, names[0], nn.Linear(16, 32))
+        setattr(self, names[1], nn.Linear(32, 16))
+        self.names = names
+        self.activation_fn = act if act is not None else nn.GELU()
+        if dropout is not None:
+            self.dropout = nn.Dropout(dropout)
+
+    def forward(self, x):
+        return getattr(self, self.names[1])(self.activation_fn(getattr(self, self.names[0])(x)))
+
+
+class Gated(nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.gate_proj, self.up_proj, self.down_proj = nn.Linear(16, 32), nn.Linear(16, 32), nn.Linear(32, 16)
+        self.act_fn = nn.SiLU()
+
+
+def test_takes_what_it_should_and_reports_the_rest():
+    model = nn.ModuleDict({"gelu": Mlp(), "silu": Mlp(nn.SiLU()), "function": Mlp(torch.nn.functional.gelu), "named": Mlp(names=("c_fc", "c_proj")),
+                           "no_dropout": Mlp(dropout=0.0), "dropout": Mlp(dropout=0.1), "tanh": Mlp(nn.GELU(approximate="tanh")),
+                           "relu": Mlp(nn.ReLU()), "gated": Gated()})
+    skipped = []
+    assert adapters.patch_mlp_epilogues(model, skipped=skipped) == 5
+    assert sorted(n for n, _ in skipped) == ["dropout", "relu", "tanh"]
+    assert "forward" not in model["gated"].__dict__ and "forward" in model["gelu"].__dict__
+
+
+def test_own_forward_off_the_gpu_and_restore():
+    model = Mlp()
+    x = torch.randn(3, 16)
+    want = model(x)
+    assert adapters.patch_mlp_epilogues(model) == 1 and adapters.patch_mlp_epilogues(model) == 1       # twice is once
+    assert torch.equal(model(x), want)
+    assert adapters.restore(model) == 1 and "forward" not in model.__dict__ and torch.equal(model(x), want)
