@@ -712,23 +712,38 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     if (ok) {
         const int output = output0 + 4 * lane;
         const int warps = kSplitThreads / 32 * p.split;
-        for (int t = rank * (kSplitThreads / 32) + warp; t < TOKENS && token0 + t < p.m; t += warps) {
-            float z[4];
+        constexpr int kRows = TOKENS >= 64 ? 2 : 1;            // rows in hand: their reads overlap
+#pragma unroll 1
+        for (int first = rank * (kSplitThreads / 32) + warp; first < TOKENS && token0 + first < p.m; first += kRows * warps) {
+            float z[kRows][4];
             if (p.split > 1) {
-                const uint32_t mine = smem_u32(&partial[t][4 * lane]);
-                float4 part[kMaxSplit];
+                float4 part[kRows][kMaxSplit];
 #pragma unroll
-                for (int r = 0; r < kMaxSplit; ++r)
-                    if (r < p.split) part[r] = load_cluster(map_to_cta(mine, uint32_t(r)));
-                z[0] = part[0].x, z[1] = part[0].y, z[2] = part[0].z, z[3] = part[0].w;
+                for (int i = 0; i < kRows; ++i) {
+                    const uint32_t mine = smem_u32(&partial[min(first + i * warps, TOKENS - 1)][4 * lane]);
 #pragma unroll
-                for (int r = 1; r < kMaxSplit; ++r)
-                    if (r < p.split) z[0] += part[r].x, z[1] += part[r].y, z[2] += part[r].z, z[3] += part[r].w;
+                    for (int r = 0; r < kMaxSplit; ++r)
+                        if (r < p.split) part[i][r] = load_cluster(map_to_cta(mine, uint32_t(r)));
+                }
+#pragma unroll
+                for (int i = 0; i < kRows; ++i) {
+                    z[i][0] = part[i][0].x, z[i][1] = part[i][0].y, z[i][2] = part[i][0].z, z[i][3] = part[i][0].w;
+#pragma unroll
+                    for (int r = 1; r < kMaxSplit; ++r)
+                        if (r < p.split) z[i][0] += part[i][r].x, z[i][1] += part[i][r].y, z[i][2] += part[i][r].z, z[i][3] += part[i][r].w;
+                }
             } else {
-                const float4 v = *reinterpret_cast<const float4*>(&partial[t][4 * lane]);
-                z[0] = v.x, z[1] = v.y, z[2] = v.z, z[3] = v.w;
+#pragma unroll
+                for (int i = 0; i < kRows; ++i) {
+                    const float4 v = *reinterpret_cast<const float4*>(&partial[min(first + i * warps, TOKENS - 1)][4 * lane]);
+                    z[i][0] = v.x, z[i][1] = v.y, z[i][2] = v.z, z[i][3] = v.w;
+                }
             }
-            if (output < p.n) finish<DT, ACT, SLOPE>(p, z, token0 + t, output);
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                const int t = first + i * warps;
+                if (t < TOKENS && token0 + t < p.m && output < p.n) finish<DT, ACT, SLOPE>(p, z[i], token0 + t, output);
+            }
         }
     }
     if (p.split > 1) {                            // the partial sums stay until the whole cluster has read them
@@ -927,6 +942,12 @@ int launch_pair(const Product& q, LinearParams& p, const DeviceInfo& dev, cudaSt
     return cuda_status(launch_early(linear_pair_kernel<DT, ACT, SLOPE, A_MN, B_MN>, unsigned(2 * pairs), kPairThreads, smem, 0u, stream, map_a, map_b, p));
 }
 
+// Whether a block of the few-row form takes all of an SM's shared memory: where every block can have an SM to itself (clusters do
+// not pack into every last one: 16 clusters of 8 or 48 of 3 took two rounds); else it takes half.
+bool alone_on_sm(int64_t blocks, int split, int sm_count) {
+    return split == 1 ? blocks <= sm_count : split <= 4 && blocks <= sm_count * 7 / 8;
+}
+
 // B, the tokens' operand, becomes the column side: D is written row by row as [tokens, outputs] all the same
 template <int DT, int ACT, bool SLOPE, int TOKENS, bool W_MN>
 int launch_split(const Product& q, LinearParams& p, const DeviceInfo& dev, int split, cudaStream_t stream) {
@@ -938,10 +959,8 @@ int launch_split(const Product& q, LinearParams& p, const DeviceInfo& dev, int s
     p.split = split;
     const int64_t blocks = int64_t(p.m_tiles) * p.n_tiles * split;
     if (blocks > 0x7fffffff) return FPT_ERR_BAD_SIZE;
-    // all the shared memory where every block can have an SM to itself (clusters do not pack into every last one: 16 clusters
-    // of 8 or 48 of 3 took two rounds), else two blocks an SM
     const uint32_t stage = kTileBytes + TOKENS * 128;
-    const uint32_t budget = (split == 1 ? blocks <= dev.sm_count : split <= 4 && blocks <= dev.sm_count * 7 / 8) ? 216u * 1024u : 108u * 1024u;
+    const uint32_t budget = alone_on_sm(blocks, split, dev.sm_count) ? 216u * 1024u : 108u * 1024u;
     p.ring = int(std::min<uint32_t>(kMaxRing, budget / stage));
     const size_t smem = 1024 + kSplitRingOffset + std::max<size_t>(size_t(p.ring) * stage, size_t(TOKENS) * 512);
     return cuda_status(launch_early(linear_split_kernel<DT, ACT, SLOPE, TOKENS, W_MN>, unsigned(blocks), kSplitThreads, smem,
@@ -950,8 +969,9 @@ int launch_split(const Product& q, LinearParams& p, const DeviceInfo& dev, int s
 
 // Which form, by the time it should take, in nanoseconds.  The terms were fitted to a sweep of both forms over six layers (512 x
 // 512 to 14336 x 4096, 1 to 1024 rows); the picks lie within some 5 % of the best measured.
-//   few rows   3000 to start and end, 28 per token of a tile (read-out), 300 for a cluster; the stream takes the longest of 210
-//              per K block and block on an SM, the weight at 6 TB/s and the tiles at 14 TB/s
+//   few rows   3000 to start and end, 20 per token of a tile (read-out), 300 + 40 a block for a cluster; the stream takes the longest
+//              of 210 per K block and block on an SM (alone: and a third per token), of 1800 per turn of the ring where a block has half the memory, of the
+//              weight at 6 TB/s and of the tiles at 14 TB/s
 //   pairs      3600 + 9.5 per column to start, read out and end; 110 + 0.95 per column per K block and round
 // Clusters of five and seven are left out: seven blocks do not pack into a processing cluster of the chip (twice the time).
 struct Form {
@@ -976,9 +996,11 @@ Form choose_form(const Product& q, int k_blocks, int sm_count) {
             if (split_key <= 0 && (split == 5 || split == 7)) continue;
             // one round of blocks, with room for the larger clusters to find their place
             if (split > 1 && blocks > (split > 2 ? 256 * sm_count / 148 : 2 * sm_count) && split_key <= 0) break;
-            const int64_t issue = 210 * per_sm * ((kb + split - 1) / split);
+            const int64_t turn = 1800 / std::min<int64_t>(kMaxRing, 108 * 1024 / (kTileBytes + tokens * 128));
+            const int64_t block = alone_on_sm(blocks, split, sm_count) ? 210 + tokens / 3 : std::max(210 * per_sm, turn);
+            const int64_t issue = block * ((kb + split - 1) / split);
             const int64_t weight = q.n * q.k * 2 / 6000, traffic = tiles * kb * (16384 + 128 * tokens) / 14000;
-            const int64_t time = 3000 + 28 * tokens + (split > 1 ? 300 : 0) + std::max(issue, std::max(weight, traffic));
+            const int64_t time = 3000 + 20 * tokens + (split > 1 ? 300 + 40 * split : 0) + std::max(issue, std::max(weight, traffic));
             if (time < least) {
                 least = time;
                 best = Form{tokens, split};
