@@ -327,7 +327,7 @@ __device__ __forceinline__ uint32_t load_position(const QkRopeArgs& a, uint32_t 
     const uint32_t b = a.seq.div(token), s = token - b * a.seq.d;
     if (!a.positions) return s;
     const int64_t from = int64_t(a.axis[pair]) * a.pos_axis + int64_t(b) * a.pos_b + int64_t(s) * a.pos_s;
-    return static_cast<const uint32_t*>(a.positions)[from * a.pos_words];                // low word
+    return __ldg(static_cast<const uint32_t*>(a.positions) + from * a.pos_words);        // low word
 }
 // where the sine and cosine of a pair lie among those of its token
 template <int C, bool HALVES>
@@ -345,9 +345,16 @@ __device__ __forceinline__ void put_trig(Shared& sm, const QkRopeArgs& a, uint32
 template <int C, bool HALVES>
 __device__ __forceinline__ void fill_trig(Shared& sm, const QkRopeArgs& a, uint32_t token0, uint32_t count) {
     const uint32_t n = count * a.pairs.d;
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-        const uint32_t t = a.pairs.div(i), pair = i - t * a.pairs.d;
-        put_trig(sm, a, t * a.pairs.d + trig_place<C, HALVES>(a, pair), load_position(a, token0 + t, pair) * a.increments[pair]);
+    for (uint32_t first = threadIdx.x; first < n; first += 2 * kThreads) {
+        uint32_t at[2], phase[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {              // both loads before either sine
+            const uint32_t i = min(first + e * kThreads, n - 1), t = a.pairs.div(i), pair = i - t * a.pairs.d;
+            at[e] = t * a.pairs.d + trig_place<C, HALVES>(a, pair);
+            phase[e] = load_position(a, token0 + t, pair) * __ldg(a.increments + pair);
+        }
+        put_trig(sm, a, at[0], phase[0]);
+        if (first + kThreads < n) put_trig(sm, a, at[1], phase[1]);
     }
 }
 // The rows of a tile by 32-bit offsets: from the first token's row where a tile is one token, else from its batch entry
