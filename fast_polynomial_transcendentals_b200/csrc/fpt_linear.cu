@@ -10,14 +10,17 @@
 // TMA into 128-byte-swizzled tiles: K-major tiles of [rows x 64 k], or MN-major ones of two panels [64 k x 64 rows], so
 // that no operand is ever transposed in memory.  Two forms:
 //
-//   linear_pair_kernel    many rows.  Persistent pairs of CTAs (cta_group::2), output tiles of 256 rows x 64 .. 256 columns, two accumulators in
-//                         turn so that the epilogue of one tile runs under the products of the next; bound by the tensor
-//                         pipe (and, in long runs, by the power cap).
+//   linear_pair_kernel    many rows.  Persistent pairs of CTAs (cta_group::2), output tiles of 256 rows x 64 .. 256 columns, two
+//                         accumulators in turn so that the epilogue of one tile runs under the products of the next; bound by
+//                         the tensor pipe (and, in long runs, by the power cap).  Measured: 4096 x 4096 -> 14336 bf16 with
+//                         GELU and bias 306 us = 1573 TFLOP/s alone, tensor pipe 91 % busy; 1999 x 1408 -> 2048 fp16 with SiLU,
+//                         bias and residual 17.9 us (one tile a pair: its parts follow one another).
 //   linear_split_kernel   few rows.  The weight is the 128-row operand and the tokens are the columns (16 .. 128 of them): a
-//                         block streams a [128 x K / split] slab of the weight through a ring of TMA tiles, two blocks per
-//                         SM; the blocks of a cluster share an output tile along K and add their fp32 partial sums over
+//                         block streams a [128 x K / split] slab of the weight through a ring of TMA tiles, one or two blocks
+//                         per SM; the blocks of a cluster share an output tile along K and add their fp32 partial sums over
 //                         distributed shared memory, in rank order (no atomics, no workspace, one launch).  Bound by the
-//                         weight's bytes.
+//                         weight's bytes: 1 row of 4096 -> 14336 bf16 21.7 us = 5.4 TB/s, 48 rows of 14336 -> 4096 24.6 us.
+//   linear_grad_act_kernel  6 bytes a value: 4096 x 4096 bf16 21 us.
 //
 // Rounding: the epilogue works on the fp32 accumulators and rounds once.  The slope act' is kept in fp16 also beside bf16
 // data: it lies in about [-0.13, 1.13], where fp16 has eight times the resolution of bf16 at the same size, so the backward
@@ -969,9 +972,9 @@ int launch_split(const Product& q, LinearParams& p, const DeviceInfo& dev, int s
 
 // Which form, by the time it should take, in nanoseconds.  The terms were fitted to a sweep of both forms over six layers (512 x
 // 512 to 14336 x 4096, 1 to 1024 rows); the picks lie within some 5 % of the best measured.
-//   few rows   3000 to start and end, 20 per token of a tile (read-out), 300 + 40 a block for a cluster; the stream takes the longest
-//              of 210 per K block and block on an SM (alone: and a third per token), of 1800 per turn of the ring where a block has half the memory, of the
-//              weight at 6 TB/s and of the tiles at 14 TB/s
+//   few rows   3000 to start and end, 20 per token of a tile (read-out), 300 + 40 a block for a cluster; the stream takes the
+//              longest of 210 per K block and block on an SM (alone: and a third per token), of 1800 per turn of the ring where
+//              a block has half the memory, of the weight at 6 TB/s and of the tiles at 14 TB/s
 //   pairs      3600 + 9.5 per column to start, read out and end; 110 + 0.95 per column per K block and round
 // Clusters of five and seven are left out: seven blocks do not pack into a processing cluster of the chip (twice the time).
 struct Form {

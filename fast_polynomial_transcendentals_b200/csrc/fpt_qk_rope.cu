@@ -8,8 +8,8 @@
 //
 // Angles: the phase of pair i is position * increment_i in 32-bit integers, where one turn is 2^32.  The product wraps as
 // the angle does, so the reduction to one turn costs nothing and is exact at every position, and of a 64-bit position only
-// the low word is needed.  sine and cosine come from sincospif on phase / 2^31.  All arithmetic is fp32; values are
-// rounded once, when they are stored.
+// the low word is needed.  Sine and cosine are Taylor series on the exact remainder from the nearest quarter turn.  All
+// arithmetic is fp32; values are rounded once, when they are stored.
 //
 // Work split: a lane holds two runs of C dimensions of a head (C = 8 where the sizes are multiples of it, else 4), placed so
 // that whole pairs lie in one lane under either pairing; a group of 4 .. 32 lanes holds a head, and the mean is a shuffle
@@ -18,6 +18,8 @@
 // once and walks over the heads with them.  The passes are bound by memory traffic, 2 (forward) or 3 (backward) values per
 // value of q and k, once instructions and shared-memory reads are few enough: pairs are kept as two fp32 vectors (first
 // members, second members), which costs nothing to unpack, and handled by the two-wide fp32 instructions.
+// Measured, 2 x 4096 tokens x (32 + 8) heads x 128 bf16: forward with the norm 29.2 us = 5.7 TB/s, backward 55 us = 4.6 TB/s
+// (bound by instruction issue at 16 warps an SM); rotation alone of 15840 such tokens 50.0 us = 6.5 TB/s.
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -36,7 +38,8 @@ constexpr int kMaxAxes = 4;
 constexpr int kStages = 3;              // items of a thread in its ring
 constexpr int kBwdTrig = 512;           // tokens x pairs of a tile of the backward pass (two entries a thread, two tiles)
 // Blocks an SM holds, by registers (16-bit data; 2 in fp32).  Measured: the forward pass with the norm 29.5 us at 3 and 33.3 at 4
-// (which spills), the rotation alone 51.8 at 3 and 50.8 at 4, the backward pass 73 at 3 (spills) and 56 at 2.
+// (which spills), the rotation alone 51.8 at 3 and 50.8 at 4, forward and backward pass together 121 with the backward
+// pass at 3 (spills) and 87 at 2.
 template <class T, bool NORM>
 constexpr int kFwdBlocks = sizeof(T) == 4 ? 2 : NORM ? 3 : 4;
 constexpr int kBwdBlocks = 2;
@@ -384,18 +387,10 @@ struct Angles {
     uint64_t cos[C / 2], sin[C / 2];
 };
 template <int C>
-__device__ __forceinline__ Angles<C> lane_angles(const Shared& sm, const QkRopeArgs& a, uint32_t first, uint32_t unit, bool turns) {
-    Angles<C> r;
-    if (turns) {
-        load_lane<C>(r.cos, sm.cos + first, unit, a.pairs.d);
-        load_lane<C>(r.sin, sm.sin + first, unit, a.pairs.d);
-    } else {                                       // dimensions behind the last pair: no rotation
-#pragma unroll
-        for (int j = 0; j < C / 2; ++j) {
-            r.cos[j] = two(1.0f, 1.0f);
-            r.sin[j] = two(0.0f, 0.0f);
-        }
-    }
+__device__ __forceinline__ Angles<C> lane_angles(const Shared& sm, const QkRopeArgs& a, uint32_t first, uint32_t unit) {
+    Angles<C> r;                                   // lanes that do not turn read the first lane's
+    load_lane<C>(r.cos, sm.cos + first, unit < uint32_t(a.rotary_units) ? unit : 0u, a.pairs.d);
+    load_lane<C>(r.sin, sm.sin + first, unit < uint32_t(a.rotary_units) ? unit : 0u, a.pairs.d);
     return r;
 }
 template <int C>
@@ -408,7 +403,7 @@ __device__ __forceinline__ Pairs<C> lane_weights(const float (&weight)[2][kMaxPa
 
 // every pair (a, b) -> scale (a cos - b sin, b cos + a sin)
 template <int C, bool SCALED>
-__device__ __forceinline__ void rotate(Pairs<C>& v, const Angles<C>& angles, float scale) {
+__device__ __forceinline__ void turn_pairs(Pairs<C>& v, const Angles<C>& angles, float scale) {
     const uint64_t plus = two(scale, scale), minus = two(-scale, -scale);
 #pragma unroll
     for (int j = 0; j < C / 2; ++j) {
@@ -421,6 +416,24 @@ __device__ __forceinline__ void rotate(Pairs<C>& v, const Angles<C>& angles, flo
         const uint64_t y = fma2(v.b[j], n, mul2(v.a[j], c));
         v.b[j] = fma2(v.a[j], s, mul2(v.b[j], c));
         v.a[j] = y;
+    }
+}
+// The same where there may be dimensions behind the last pair, which are not mixed (a rotation by nothing would carry an
+// infinity over as infinity x 0).  Heads that rotate as a whole take a branch that is the same for the launch: asking every
+// lane costs 1.5 % of the passes.
+template <int C, bool SCALED>
+__device__ __forceinline__ void rotate(Pairs<C>& v, const Angles<C>& angles, float scale, const QkRopeArgs& a, bool turns) {
+    if (a.rotary_units == a.units) {
+        turn_pairs<C, SCALED>(v, angles, scale);
+    } else if (turns) {
+        turn_pairs<C, SCALED>(v, angles, scale);
+    } else if constexpr (SCALED) {
+        const uint64_t plus = two(scale, scale);
+#pragma unroll
+        for (int j = 0; j < C / 2; ++j) {
+            v.a[j] = mul2(v.a[j], plus);
+            v.b[j] = mul2(v.b[j], plus);
+        }
     }
 }
 template <int C>
@@ -504,7 +517,8 @@ __global__ void __launch_bounds__(kThreads, (kFwdBlocks<T, NORM>)) qk_rope_kerne
         keep_weight<C>(sm.weight[1], a, weight[1]);
     }
     __syncthreads();
-    const Angles<C> angles = lane_angles<C>(sm, a, slot * a.pairs.d, unit, unit < a.rotary_units);
+    const Angles<C> angles = lane_angles<C>(sm, a, slot * a.pairs.d, unit);
+    const bool turns = unit < a.rotary_units;
     Pairs<C> w;
     if constexpr (NORM) w = lane_weights<C>(sm.weight[head >= q_heads], a, unit);
     bool keys = head >= q_heads;                   // whose weights w holds
@@ -532,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, (kFwdBlocks<T, NORM>)) qk_rope_kerne
             r = rsqrtf(fmaf(group_sum<G>(live ? (sa.x + sa.y) + (sb.x + sb.y) : 0.0f), inv_dim, a.eps));
             v = times(v, w);
         }
-        rotate<C, NORM>(v, angles, r);
+        rotate<C, NORM>(v, angles, r, a, turns);
         if (!live || h >= end) continue;
         const Raw<T, C> y = pack<T, C, HALVES>(v);
         char* out = key ? ok : oq;
@@ -556,6 +570,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_norm_rope_bwd_kernel(
     const int lane_unit = threadIdx.x & (G - 1);
     const bool live = lane_unit < a.units;
     const int unit = live ? lane_unit : 0;
+    const bool turns = unit < a.rotary_units;
     const Place at = place<C>(unit, a.rotary_units);
     const uint32_t lo = uint32_t(at.lo) * sizeof(T), hi = uint32_t(at.hi) * sizeof(T), out_bytes = uint32_t(a.dim) * sizeof(T);
     const float inv_dim = 1.0f / float(a.dim);
@@ -630,14 +645,14 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_norm_rope_bwd_kernel(
         const uint32_t slot = min(my_slot, count - 1), end = my_slot < count ? heads : 0u;
         char* out = static_cast<char*>(side.out) + int64_t(token0) * heads * out_bytes;
         load_positions(tile + side.blocks);
-        const Angles<C> angles = lane_angles<C>(sm, a, half * kBwdTrig + slot * a.pairs.d, unit, unit < a.rotary_units);
+        const Angles<C> angles = lane_angles<C>(sm, a, half * kBwdTrig + slot * a.pairs.d, unit);
 #pragma unroll 1
         for (uint32_t n = 0; n < rounds; ++n) {
             fetch();
             copy_wait<kAhead>();
             const uint32_t i = head + n * step;
             Pairs<C> g = unpack<T, C, HALVES>(ring_g.read(stage));
-            rotate<C, false>(g, angles, 1.0f);
+            rotate<C, false>(g, angles, 1.0f, a, turns);
             const Pairs<C> f = unpack<T, C, HALVES>(ring_x.read(stage)), h = times(g, lane_weights<C>(sm.weight[0], a, unit));
             stage = stage + 1 == kStages ? 0 : stage + 1;
             uint64_t ssa = 0, ssb = 0, da = 0, db = 0;
@@ -748,7 +763,8 @@ int group_lanes(int units) {
     return g;
 }
 
-// Tokens of a tile, a power of two: every group gets at least `rounds` heads of its token.
+// Tokens of a tile, a power of two: every group gets at least `rounds` heads of its token.  Measured for the forward pass (the
+// shapes above, us at 2, 4, 8 heads): with the norm 37.3, 29.0, 29.6; rotation alone 55.9, 50.0, 51.2.
 uint32_t tile_tokens(uint32_t groups, uint32_t heads, uint32_t pairs, uint32_t rounds, uint32_t trig) {
     uint32_t t = 1;
     while (2 * t <= std::min<uint32_t>(kMaxTileTokens, groups) && 2 * t * pairs <= trig && t * heads < rounds * groups) t *= 2;
@@ -871,11 +887,14 @@ extern "C" int fpt_qk_rope(void* q_out, void* k_out, const void* q, const void* 
     if (int rc = current_device_info(&dev)) return rc;
     a.eps = eps;
     a.sin_sign = inverse ? 0x80000000u : 0u;
-    // One head per group and block while that gives no more than a few blocks per SM (single tokens: the shortest chain
-    // of loads); beyond it a block takes all heads of as many tokens as leave every group at least four heads.
+    // One head per group and block while all blocks are resident at once (single tokens: the shortest chain of loads); beyond
+    // it a block takes all heads of as many tokens as leave every group at least four heads.  Measured with 32 + 8 heads of
+    // 128 in bf16, us one way and the other: 4 tokens 2.4 / 3.8, 128 tokens 3.5 / 4.0, 256 tokens (not resident) 4.9 / 4.1,
+    // 512 tokens 7.3 / 4.3; rotation alone, 256 tokens (resident) 3.1 / 3.3.
     const uint32_t groups = uint32_t(kThreads / (norm ? group_lanes(a.units) : a.units)), heads = a.side[0].heads + a.side[1].heads;
     a.groups = groups;
-    const bool few = uint64_t(a.tokens) * heads <= uint64_t(groups) * uint64_t(dev.sm_count) * 4;
+    const uint32_t resident = uint32_t(dev.sm_count * (dtype == FPT_FP32 ? kFwdBlocks<float, true> : norm ? kFwdBlocks<__half, true> : kFwdBlocks<__half, false>));
+    const bool few = uint64_t(a.tokens) * ((heads + groups - 1) / groups) <= resident;
     a.tile_tokens = few ? 1u : tile_tokens(groups, heads, uint32_t(pairs), 4, kMaxTrig);
     for (const Side& s : a.side)
         if (!reach(s.xs, seq, s.heads, a.tile_tokens)) a.tile_tokens = 1u;

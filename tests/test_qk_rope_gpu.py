@@ -264,6 +264,36 @@ def test_zero_rows_and_rows_that_are_not_numbers(cuda):
         assert torch.equal(a[keep], b[keep])
 
 
+@pytest.mark.parametrize("dim, pairs", [(64, 16), (40, 4), (128, 32)])
+@pytest.mark.parametrize("pairing", ["adjacent", "halves"])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_dimensions_behind_the_pairs_are_not_mixed(cuda, dtype, pairing, dim, pairs):
+    """The rotation alone passes them through, infinities and -0 bit for bit and NaN as NaN (the conversion to 16 bits gives it
+    one payload), and so does its gradient; under the norm one that is not finite makes NaN of itself only."""
+    bits = torch.int32 if dtype == "fp32" else torch.int16
+    inc, pos = rope_phase_increments(2 * pairs, device=cuda), torch.arange(6, device=cuda)[None]
+
+    def spoiled(seed):
+        out = make(1, 6, 4, 2, dim, DTYPES[dtype], cuda, seed=seed)
+        for t in out:
+            t[0, 1, 1, 2 * pairs + 1] = math.inf
+            t[0, 2, 0, 2 * pairs + 4] = math.nan
+            t[0, 3, 1, dim - 1] = -math.inf
+            t[0, 4, :, 2 * pairs:] = -0.0
+        return out
+    x, dy = [t.requires_grad_() for t in spoiled(3)], spoiled(4)
+    y = qk_rope.rope_axes(*x, inc, pos, [pairs], pairing=pairing)
+    for got, want in (*zip(y, x), *zip(torch.autograd.grad(y, x, dy), dy)):
+        a, b = (t.detach()[..., 2 * pairs:].contiguous() for t in (got, want))
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.view(bits)[~a.isnan()], b.view(bits)[~a.isnan()])
+        assert torch.isfinite(got[..., :2 * pairs]).all()
+    turn = turns(inc, None, 1, 6)
+    with torch.no_grad():
+        for got, t in zip(qk_rope.qk_norm_rope(*x, None, None, inc, pairing=pairing), x):
+            want, _ = plain_norm(t, None, turn, pairing, 1e-6)
+            assert torch.equal(got.isnan().cpu(), want.isnan())
+
+
 @pytest.mark.parametrize("batch, seq", [(0, 5), (3, 0)])
 def test_nothing_to_do(cuda, batch, seq):
     q, k = (torch.empty(batch, seq, h, 64, device=cuda, dtype=torch.bfloat16, requires_grad=True) for h in (4, 2))
