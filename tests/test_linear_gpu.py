@@ -265,6 +265,20 @@ def test_no_second_gradient(cuda):
         torch.autograd.grad(linear_act(x, w, activation="gelu").float().sum(), [x], create_graph=True)
 
 
+def test_tail_of_gelu(cuda):
+    """Relative to the result, where GELU(z) is small: z = x exactly (identity weight), so what is left is half a step of the
+    dtype (fp16: at least 2^-25), the fit of the tail (1e-6) and its exponential, whose argument of at most 15 is rounded by
+    2^-21 and twice 2^-24 of it (3e-6 together): (1 + 2^-10) h + 4e-6."""
+    weight = torch.eye(64, device=cuda)
+    for dtype in DTYPES.values():
+        z = (-torch.arange(64 * 64, device=cuda).double() / (64 * 64) * 5.4).reshape(64, 64).to(dtype)
+        want = z.double() * torch.special.ndtr(z.double())
+        rel, least = half(dtype)
+        for x in (z, z[:3]):
+            got = linear_act(x, weight.to(dtype), activation="gelu").double()
+            assert ((got - want[:len(x)]).abs() <= ((1 + 2.0 ** -10) * rel + 4e-6) * want[:len(x)].abs() + least).all()
+
+
 def test_values_that_are_not_finite_stay_in_their_row(cuda):
     for rows in (9, 300):
         x, w, b, r, _ = inputs(rows, 64, 136, torch.bfloat16, cuda)
