@@ -14,7 +14,7 @@
 //                         accumulators in turn so that the epilogue of one tile runs under the products of the next; bound by
 //                         the tensor pipe (and, in long runs, by the power cap).  Measured: 4096 x 4096 -> 14336 bf16 with
 //                         GELU and bias 306 us = 1573 TFLOP/s alone, tensor pipe 91 % busy; 1999 x 1408 -> 2048 fp16 with SiLU,
-//                         bias and residual 17.9 us (one tile a pair: its parts follow one another).
+//                         bias and residual 17.7 us (one tile a pair: its parts follow one another).
 //   linear_split_kernel   few rows.  The weight is the 128-row operand and the tokens are the columns (16 .. 128 of them): a
 //                         block streams a [128 x K / split] slab of the weight through a ring of TMA tiles, one or two blocks
 //                         per SM; the blocks of a cluster share an output tile along K and add their fp32 partial sums over
@@ -1163,7 +1163,8 @@ extern "C" int fpt_linear_grad_weight(void* dw, const void* dz, const void* x, i
 }
 
 namespace {
-// rows one block sums: enough blocks for every SM several times over, at least 32 rows each
+// rows one block sums: some six blocks for each of 148 SMs (a constant: the size of the workspace does not ask for a device), at
+// least 32 rows each
 int grad_act_chunk(int64_t rows, int64_t out) {
     const int64_t column_blocks = (out + kActColumns - 1) / kActColumns;
     const int64_t chunks = std::max<int64_t>(1, 148 * 6 / column_blocks);

@@ -246,6 +246,13 @@ def _epilogue_activation(fn: Any) -> str | None:
     return {"geluactivation": "gelu", "siluactivation": "silu"}.get(type(fn).__name__.lower())
 
 
+def _as_it_comes(*modules: Any) -> bool:
+    """Whether calling these does what their class does: no hooks, and for projections nn.Linear's own forward (a subclass or an
+    instance with another one computes something else)."""
+    return not any(isinstance(m, nn.Module) and (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                   or (isinstance(m, nn.Linear) and (type(m).forward is not nn.Linear.forward or "forward" in m.__dict__))) for m in modules)
+
+
 def patch_mlp_epilogues(model: nn.Module, *, variant: str = "native", degree: int | None = None, coeff_source: str = "current",
                         skipped: list[tuple[str, str]] | None = None) -> int:
     """down(act(up(x))) as two kernels, bias and activation in the first one's epilogue and the bias in the second's
@@ -253,9 +260,10 @@ def patch_mlp_epilogues(model: nn.Module, *, variant: str = "native", degree: in
 
     A module qualifies by structure: two `nn.Linear` under the usual names (`fc1 / fc2`, `up_proj / down_proj` without a gate,
     ...), an erf GELU or SiLU in an activation slot, and nothing else that could act in between (dropout only where its
-    probability is zero); others with the two projections are left alone and reported through `skipped`.  variant "native"
-    evaluates the activation in fp32, "polynomial" runs the packed program (degree 5 for GELU, 3 for SiLU by default).
-    Inputs that are not float16 or bfloat16 on the GPU, or whose width is no multiple of 8, take the module's own forward."""
+    probability is zero, no parameters of the module's own); others with the two projections are left alone and reported through
+    `skipped`.  variant "native" evaluates the activation in fp32, "polynomial" runs the packed program (degree 5 for GELU, 3
+    for SiLU by default).  Inputs that are not float16 or bfloat16 on the GPU, or whose width is no multiple of 8, and
+    projections with hooks or a forward of their own (adapters on top of them) take the module's own forward."""
     patched = 0
     for name, module in model.named_modules():
         pair = next((p for p in _MLP_PAIRS if all(isinstance(getattr(module, n, None), nn.Linear) for n in p)), None)
@@ -265,6 +273,7 @@ def patch_mlp_epilogues(model: nn.Module, *, variant: str = "native", degree: in
         activation = _epilogue_activation(getattr(module, slot)) if slot else None
         others = [n for n, m in module.named_children() if n not in (*pair, slot)
                   and not isinstance(m, nn.Identity) and not (isinstance(m, nn.Dropout) and m.p == 0)]
+        others += [n for n, p in module.named_parameters(recurse=False) if p is not None]
         if activation is None or others:
             if skipped is not None:
                 skipped.append((name, f"also holds {', '.join(others)}" if others else
@@ -272,10 +281,11 @@ def patch_mlp_epilogues(model: nn.Module, *, variant: str = "native", degree: in
             continue
         chosen = 0 if variant == "native" else degree if degree is not None else {"gelu": 5, "silu": 3}[activation]
 
-        def forward(self, x, *args, _up=pair[0], _down=pair[1], _act=activation, _degree=chosen, **kwargs):
+        def forward(self, x, *args, _up=pair[0], _down=pair[1], _slot=slot, _act=activation, _degree=chosen, **kwargs):
             up, down = getattr(self, _up), getattr(self, _down)
             if not (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and up.weight.dtype == down.weight.dtype == x.dtype
-                    and up.weight.shape[1] % 8 == 0 and down.weight.shape[1] % 8 == 0) or torch.is_autocast_enabled("cuda"):
+                    and up.weight.shape[1] % 8 == 0 and down.weight.shape[1] % 8 == 0
+                    and _as_it_comes(up, down, getattr(self, _slot))) or torch.is_autocast_enabled("cuda"):
                 return self.__dict__[_ORIGINAL](x, *args, **kwargs)
             hidden = linear_act(x, up.weight, up.bias, activation=_act, degree=_degree, coeff_source=coeff_source)
             return linear_act(hidden, down.weight, down.bias)

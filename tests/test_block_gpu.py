@@ -188,6 +188,16 @@ def test_adapter_runs_the_feed_forward(cuda, act, dtype):
     check_linear_status()
 
 
+def test_adapter_leaves_hooked_projections_alone(cuda):
+    model = Mlp(nn.GELU()).to(cuda, BF)
+    x = torch.randn(5, model.fc1.in_features, device=cuda).to(BF)
+    model.fc1.register_forward_hook(lambda module, args, out: 2 * out)
+    with torch.no_grad():
+        want = model(x)
+        assert adapters.patch_mlp_epilogues(model) == 1
+        assert torch.equal(model(x), want)
+
+
 def test_offsets_past_31_bits(cuda):
     """Results of more than 2^31 elements, rows checked at both ends and in between.  One rounding to bf16 (eps / 2 = 2^-8 of
     the value: eight significant bits) and fp32 sums of 64 terms of size 64 / 8 in all (18 u S, S < 100: below 3e-4)."""

@@ -43,3 +43,25 @@ def test_own_forward_off_the_gpu_and_restore():
     assert adapters.patch_mlp_epilogues(model) == 1 and adapters.patch_mlp_epilogues(model) == 1       # twice is once
     assert torch.equal(model(x), want)
     assert adapters.restore(model) == 1 and "forward" not in model.__dict__ and torch.equal(model(x), want)
+
+
+def test_own_parameters_keep_a_module_as_it_is():
+    model = Mlp()
+    model.scale = nn.Parameter(torch.ones(16))
+    skipped = []
+    assert adapters.patch_mlp_epilogues(model, skipped=skipped) == 0
+    assert skipped == [("", "also holds scale")]
+
+
+def test_hooks_and_forwards_of_the_projections_are_seen():
+    class Scaled(nn.Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    plain, hooked, scaled, bound = Mlp(), Mlp(), Mlp(), Mlp()
+    hooked.fc1.register_forward_hook(lambda module, args, out: 2 * out)
+    scaled.fc2 = Scaled(32, 16)
+    bound.fc1.forward = lambda x: x
+    assert adapters._as_it_comes(plain.fc1, plain.fc2, plain.activation_fn)
+    for model in (hooked, scaled, bound):
+        assert not adapters._as_it_comes(model.fc1, model.fc2, model.activation_fn)
