@@ -8,13 +8,15 @@
 //
 // All products are D[i, j] = sum_k A[i, k] B[j, k] on tcgen05 with fp32 accumulators in tensor memory, operands brought by
 // TMA into 128-byte-swizzled tiles: K-major tiles of [rows x 64 k], or MN-major ones of two panels [64 k x 64 rows], so
-// that no operand is ever transposed in memory.  Two forms:
+// that no operand is ever transposed in memory.  The forms:
 //
 //   linear_pair_kernel    many rows.  Persistent pairs of CTAs (cta_group::2), output tiles of 256 rows x 64 .. 256 columns, two
 //                         accumulators in turn so that the epilogue of one tile runs under the products of the next; bound by
 //                         the tensor pipe (and, in long runs, by the power cap).  Measured: 4096 x 4096 -> 14336 bf16 with
 //                         GELU and bias 306 us = 1573 TFLOP/s alone, tensor pipe 91 % busy; 1999 x 1408 -> 2048 fp16 with SiLU,
 //                         bias and residual 17.7 us (one tile a pair: its parts follow one another).
+//   linear_shared_pair_kernel  the same for few tiles: two or four pairs share a tile along K (dW of 512 x 512 over 16384 rows
+//                         17.9 us; 43.8 with a pair a tile).
 //   linear_split_kernel   few rows.  The weight is the 128-row operand and the tokens are the columns (16 .. 128 of them): a
 //                         block streams a [128 x K / split] slab of the weight through a ring of TMA tiles, one or two blocks
 //                         per SM; the blocks of a cluster share an output tile along K and add their fp32 partial sums over
@@ -65,7 +67,7 @@ struct LinearParams {
     int64_t out_ld, res_ld, slope_ld;
     int m, n, k_blocks;             // k_blocks: of 64 (split form), of 64 chunks (pair form)
     int m_tiles, n_tiles;
-    int split;                      // blocks per cluster (split form)
+    int split;                      // blocks (few-row form) or pairs (pair form) of a cluster, which share a tile along K
     int columns;                    // columns of an output tile (pair form), a multiple of 32
     int ring;                       // stages of the ring
     uint32_t stage_bytes;           // their size, and the K blocks of 64 in one (pair form)
@@ -377,6 +379,21 @@ __device__ __forceinline__ uint32_t tile_lo(const void* tile) { return umma_smem
 template <bool MN>
 constexpr uint32_t kStep16 = MN ? 2048u / 16u : 2u;
 
+// 16 bytes of shared memory: of any CTA of the cluster (map_to_cta), into this one's
+__device__ __forceinline__ float4 load_cluster(uint32_t address) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address) : "memory");
+    return v;
+}
+__device__ __forceinline__ float load_cluster1(uint32_t address) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(address) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_shared(uint32_t address, uint32_t x) {
+    asm volatile("st.shared.b32 [%0], %1;" :: "r"(address), "r"(x) : "memory");
+}
+
 // ---- many rows: pairs of CTAs ---------------------------------------------------------------------------------------
 
 constexpr uint32_t kRingBytes = 192 * 1024;
@@ -444,14 +461,17 @@ __device__ __forceinline__ uint32_t share_lo(uint32_t first, uint32_t k, uint32_
 
 // Each CTA of the pair holds 128 rows of A and half the tile's columns' rows of B and receives 128 rows x p.columns columns of
 // D; the hand-overs are those of gate_up_swiglu_pair_kernel.  The host picks the number of columns so that the tiles come
-// out even over the pairs.
-template <int DT, int ACT, bool SLOPE, bool A_MN, bool B_MN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
-linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ LinearParams p) {
+// out even over the pairs.  Where there are only a few tiles (SHARED), the p.split pairs of a cluster share a tile along K, one tile
+// a cluster: every CTA finishes a share of the tile's columns and lays the fp32 sums of the others' shares where its ring was,
+// a column's 128 rows together (a lane per row: with a row's columns together every lane's read from another CTA is a transfer
+// of its own, and the exchange of 256 columns took 4 us more).  The order of the additions is fixed.
+template <int DT, int ACT, bool SLOPE, bool A_MN, bool B_MN, bool SHARED>
+__device__ __forceinline__ void pair_tiles(const CUtensorMap& map_a, const CUtensorMap& map_b, const LinearParams& p) {
     extern __shared__ uint8_t smem_raw[];
     PairSmem& sm = *reinterpret_cast<PairSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_cta_rank();
+    const uint32_t cta = cluster_cta_rank(), rank = SHARED ? cta & 1u : cta, lead = SHARED ? cta & ~1u : 0u;   // rank in the pair; its first CTA
+    const int split = SHARED ? p.split : 1;
     volatile uint32_t* abort_flag = &sm.abort_flag;
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.ring; ++s) {
@@ -477,7 +497,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     const uint32_t tmem = sm.tmem_base;
     wait_for_inputs();
     const int tiles = p.m_tiles * p.n_tiles;
-    const int first_tile = blockIdx.x >> 1, tile_step = gridDim.x >> 1;
+    const int first_tile = int(blockIdx.x / uint32_t(2 * split)), tile_step = int(gridDim.x / uint32_t(2 * split));
+    const int part = SHARED ? int(cta >> 1) : 0;    // of the K blocks
+    const int kb0 = SHARED ? int(int64_t(p.k_blocks) * part / split) : 0, kb1 = SHARED ? int(int64_t(p.k_blocks) * (part + 1) / split) : p.k_blocks;
 
     if (warp == 0) {
         if (lane == 0) {
@@ -487,10 +509,10 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             const uint32_t a_bytes = share_bytes<A_MN>(128, p.chunks), bytes = 2 * (a_bytes + share_bytes<B_MN>(b_rows, p.chunks));
             for (int tile = first_tile; tile < tiles && ok; tile += tile_step) {
                 const PairTile t = pair_tile(p, tile);
-                for (int kb = 0; kb < p.k_blocks; ++kb) {
+                for (int kb = kb0; kb < kb1; ++kb) {
                     if (turn > 0) ok = wait(&sm.empty[s], (turn - 1u) & 1u, abort_flag, p.status, kWaitEmpty);
                     if (!ok) break;
-                    const uint32_t bar = map_to_cta(smem_u32(&sm.full[s]), 0);
+                    const uint32_t bar = map_to_cta(smem_u32(&sm.full[s]), lead);
                     uint8_t* stage = sm.ring + s * p.stage_bytes;
                     if (rank == 0) mbar_arrive_expect_tx(&sm.full[s], bytes);
                     load_pair<A_MN>(stage, &map_a, bar, kb, t.row0 + int(rank) * 128, 128, p.chunks, p.a_whole);
@@ -518,18 +540,18 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 }
                 tc_fence_after_sync();
             }
-            for (int kb = 0; kb < p.k_blocks; ++kb) {
+            for (int kb = kb0; kb < kb1; ++kb) {
                 ok = wait(&sm.full[s], turn & 1u, abort_flag, p.status, kWaitFull);
                 if (!ok) break;
                 tc_fence_after_sync();
                 const uint32_t a_lo = a_first + s * (p.stage_bytes / 16u), b_lo = b_first + s * (p.stage_bytes / 16u);
 #pragma unroll 4
                 for (uint32_t k = 0; k < uint32_t(p.chunks) * (kBlockK / 16); ++k)
-                    if (elected) umma_ss_words_pair(tmem + a * 256u, share_lo<A_MN>(a_lo, k, 128), share_lo<B_MN>(b_lo, k, b_rows), desc_hi, idesc, (kb > 0 || k > 0) ? 1u : 0u);
-                if (elected) umma_commit_pair(&sm.empty[s], 3);
+                    if (elected) umma_ss_words_pair(tmem + a * 256u, share_lo<A_MN>(a_lo, k, 128), share_lo<B_MN>(b_lo, k, b_rows), desc_hi, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+                if (elected) umma_commit_pair(&sm.empty[s], uint16_t(3u << lead));
                 if (++s == uint32_t(p.ring)) s = 0, ++turn;
             }
-            if (ok && elected) umma_commit_pair(&sm.acc_full[a], 3);
+            if (ok && elected) umma_commit_pair(&sm.acc_full[a], uint16_t(3u << lead));
         }
     } else if (warp >= 4) {
         // four warps hold the 128 rows (a warp reads the 32 lanes of its number modulo 4); such sets take the 32-column chunks in
@@ -537,6 +559,8 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         const uint32_t lane_base = uint32_t(32 * (warp & 3)) << 16;
         const int set = (warp - 4) >> 2;
         Stage& stage = sm.stage[warp - 4];
+        const int share = SHARED ? p.columns / split : p.columns, c_first = part * share;  // the columns this CTA finishes
+        const uint32_t sums = smem_u32(sm.ring) + uint32_t(32 * (warp & 3) + lane) * 4u;       // [column][row of 128]
         uint32_t local = 0;
         bool ok = true;
         for (int tile = first_tile; tile < tiles && ok; tile += tile_step, ++local) {
@@ -551,12 +575,27 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 if (p.residual) load_rows(res, static_cast<const uint16_t*>(p.residual) + int64_t(row0) * p.res_ld + column, p.res_ld, lane, valid);
                 if (p.bias) bias = load_any(p.bias, p.bias_dtype, column + lane);
             };
-            prefetch(t.column0 + set * 32);
+            prefetch(t.column0 + c_first + set * 32);
             ok = wait(&sm.acc_full[a], (local >> 1) & 1u, abort_flag, p.status, kWaitAccFull);
-            if (!ok) break;
             tc_fence_after_sync();
+            if constexpr (SHARED) {                 // one tile a cluster: the ring is done with
+                if (ok) {
 #pragma unroll 1
-            for (int c = set * 32; c < p.columns; c += kEpilogueWarps * 8) {
+                    for (int c = set * 32; c < p.columns; c += kEpilogueWarps * 8) {
+                        if (c >= c_first && c < c_first + share) continue;      // stays in tensor memory
+                        uint32_t acc[32];
+                        tmem_ld_32x32b_x32(tmem + lane_base + a * 256u + uint32_t(c), acc);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) store_shared(sums + uint32_t(c + i) * 512u, acc[i]);
+                    }
+                }
+                __syncwarp();
+                cluster_sync_all();                 // the other warps' is behind their part
+            }
+            if (!ok) break;
+#pragma unroll 1
+            for (int c = c_first + set * 32; c < c_first + share; c += kEpilogueWarps * 8) {
                 const int column = t.column0 + c;
                 if (column >= p.n || valid <= 0) break;
                 uint32_t acc[32];
@@ -565,10 +604,22 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 float z[32];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) z[i] = __uint_as_float(acc[i]);
+                if constexpr (SHARED) {
+#pragma unroll 1
+                    for (int q = 1; q < split; ++q) {                   // the other pairs' sums, from the next pair round
+                        const uint32_t other = (cta + 2u * uint32_t(q)) & uint32_t(2 * split - 1);      // split: a power of two
+                        const uint32_t from = map_to_cta(sums + uint32_t(c) * 512u, other);
+                        float v[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = load_cluster1(from + 512u * uint32_t(i));
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) z[i] += v[i];
+                    }
+                }
                 if (p.staged && column + 32 <= p.n) {
                     const uint4 mine[4] = {res[0], res[1], res[2], res[3]};
                     const float mine_bias = bias;
-                    prefetch(column + kEpilogueWarps * 8);
+                    if (!SHARED || c + kEpilogueWarps * 8 < c_first + share) prefetch(column + kEpilogueWarps * 8);
                     finish_staged<DT, ACT, SLOPE>(p, z, mine, mine_bias, stage, row0, column, lane);
                 } else {
                     if (lane < valid) finish<DT, ACT, SLOPE>(p, z, row0 + lane, column);
@@ -579,15 +630,29 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             __syncwarp();
             if (lane == 0) {
                 if (rank == 0) mbar_arrive(&sm.acc_empty[a]);
-                else mbar_arrive_cluster(map_to_cta(smem_u32(&sm.acc_empty[a]), 0));
+                else mbar_arrive_cluster(map_to_cta(smem_u32(&sm.acc_empty[a]), lead));
             }
         }
     }
-    // neither CTA may leave while the other can still reach its barriers or tensor memory
+    if (SHARED && warp < 4) {                       // the barrier between the sums of the cluster and their readers
+        __syncwarp();
+        cluster_sync_all();
+    }
+    // no CTA may leave while another can still reach its barriers, its tensor memory or its sums
     tc_fence_before_sync();
     __syncwarp();
     cluster_sync_all();
     if (warp == 2) tmem_dealloc_pair(tmem, 512);
+}
+template <int DT, int ACT, bool SLOPE, bool A_MN, bool B_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ LinearParams p) {
+    pair_tiles<DT, ACT, SLOPE, A_MN, B_MN, false>(map_a, map_b, p);
+}
+template <int DT, int ACT, bool SLOPE, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(kPairThreads, 1)         // clusters of 2 p.split
+linear_shared_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ LinearParams p) {
+    pair_tiles<DT, ACT, SLOPE, A_MN, B_MN, true>(map_a, map_b, p);
 }
 
 // ---- few rows: the weight streams, the tokens are columns ---------------------------------------------------------------
@@ -605,12 +670,6 @@ struct SplitSmem {
 };
 constexpr uint32_t kSplitRingOffset = 1024;
 static_assert(sizeof(SplitSmem) <= kSplitRingOffset, "barriers before the ring");
-
-__device__ __forceinline__ float4 load_cluster(uint32_t address) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(address) : "memory");
-    return v;
-}
 
 // D is [tokens, outputs] (p.m tokens, p.n outputs); A = the weight, B = the tokens.  The p.split blocks of a cluster take
 // equal runs of K blocks.
@@ -930,10 +989,46 @@ int pair_columns(const Product& q, int pairs) {
     return best;
 }
 
+// Tile width and pairs per tile, and the time it should take in nanoseconds: 3600 + 9.5 per column to start, read out and end; per
+// K block and round 1.25 per column (products), 165 + 0.36 per column (a pair's loads) or what all tiles at work draw at 14 TB/s;
+// no less than both operands at 6 TB/s.  Tiles shared along K take 1200 + 8 per column more, and all their clusters have to be
+// resident at once (32 of four CTAs, 14 of eight; 16 of eight take two rounds).
+// Measured, us on one pair a tile, the best width, and on two or four: 256 rows of 4096 -> 4096 15.8 and 14.0, 512 rows of
+// 4096 -> 4096 17.7 and 19.3, of 14336 -> 4096 53.5 and 49.1; dW of 512 x 512 over 16384 rows 43.8 and 17.9.
+struct PairForm {
+    int columns, split;
+    int64_t time;
+};
+PairForm pair_form(const Product& q, int sm_count) {
+    const int64_t stages = (q.k + kChunks * kBlockK - 1) / (kChunks * kBlockK), row_tiles = (q.m + 255) / 256;
+    const auto tiles = [&](int columns) { return row_tiles * ((q.n + columns - 1) / columns); };
+    const int64_t operands = (q.m + q.n) * q.k * 2 / 6000;
+    const auto stream = [&](int columns, int split) {                 // the K blocks of the busiest pair
+        const int64_t count = tiles(columns) * split, resident = std::min<int64_t>(count, sm_count / 2), rounds = (count + resident - 1) / resident;
+        const int64_t block = std::max<int64_t>({125 * columns / 100, 165 + 36 * columns / 100, (16384 + 64 * columns) * 2 * resident / 14000});
+        return std::max(operands, rounds * ((stages + split - 1) / split) * kChunks * block);
+    };
+    const int columns = pair_columns(q, sm_count / 2);
+    const int key = fpt::tuning_linear_tokens() == 0 ? fpt::tuning_linear_split() : 0, width = fpt::tuning_linear_columns();
+    PairForm best{columns, 1, 3600 + 95 * columns / 10 + stream(columns, 1)};
+    for (int split = 2; split <= 4; split *= 2) {
+        if (split > stages || (key > 0 && key != split)) continue;
+        for (int c = 256; c >= 64; c /= 2) {
+            if ((width > 0 && c != width) || c % (32 * split) || (q.b_mn && c % 128)) continue;
+            if (key <= 0 && tiles(c) > (split == 2 ? 32 : 14) * sm_count / 148) continue;
+            const int64_t time = 4800 + 175 * c / 10 + stream(c, split);
+            if (key > 0 || time < best.time) best = PairForm{c, split, time};
+            if (key > 0) return best;
+        }
+    }
+    return best;
+}
+
 template <int DT, int ACT, bool SLOPE, bool A_MN, bool B_MN>
-int launch_pair(const Product& q, LinearParams& p, const DeviceInfo& dev, cudaStream_t stream) {
+int launch_pair(const Product& q, LinearParams& p, const DeviceInfo& dev, PairForm form, cudaStream_t stream) {
     CUtensorMap map_a, map_b;
-    p.columns = pair_columns(q, dev.sm_count / 2);
+    p.columns = form.columns;
+    p.split = form.split;
     p.chunks = kChunks;
     p.k_blocks = int((q.k + p.chunks * kBlockK - 1) / (p.chunks * kBlockK));
     if (int rc = tile_map(&map_a, &p.a_whole, q.a, q.m, q.k, q.a_ld, A_MN, 128, p.chunks)) return rc;
@@ -944,8 +1039,13 @@ int launch_pair(const Product& q, LinearParams& p, const DeviceInfo& dev, cudaSt
     p.ring = int(std::min<uint32_t>(kMaxRing, kRingBytes / p.stage_bytes));
     p.staged = p.vec_out && (!p.residual || p.vec_res) && (!p.slope || p.vec_slope);
     static_assert(sizeof(PairSmem) + 1024 <= 227 * 1024, "shared memory budget");
+    static_assert(128 * 256 * 4 <= kRingBytes, "a CTA's sums fit its ring");
     const size_t smem = sizeof(PairSmem) + 1024;
-    const int64_t pairs = std::min<int64_t>(int64_t(p.m_tiles) * p.n_tiles, dev.sm_count / 2);
+    const int64_t tiles = int64_t(p.m_tiles) * p.n_tiles;
+    const int64_t pairs = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, dev.sm_count / 2);
+    if (pairs > 0x3fffffff) return FPT_ERR_BAD_SIZE;
+    if (p.split > 1)
+        return cuda_status(launch_early(linear_shared_pair_kernel<DT, ACT, SLOPE, A_MN, B_MN>, unsigned(2 * pairs), kPairThreads, smem, unsigned(2 * p.split), stream, map_a, map_b, p));
     return cuda_status(launch_early(linear_pair_kernel<DT, ACT, SLOPE, A_MN, B_MN>, unsigned(2 * pairs), kPairThreads, smem, 0u, stream, map_a, map_b, p));
 }
 
@@ -975,20 +1075,19 @@ int launch_split(const Product& q, LinearParams& p, const DeviceInfo& dev, int s
 }
 
 // Which form, by the time it should take, in nanoseconds.  The terms were fitted to a sweep of both forms over six layers (512 x
-// 512 to 14336 x 4096, 1 to 1024 rows); the picks lie within some 5 % of the best measured.
+// 512 to 14336 x 4096, 1 to 1024 rows); the picks lie within some 5 % of the best measured, in a few places 20 % (256 rows of
+// 8192 -> 1024 16.5 us, on shared tiles 13.6).
 //   few rows   3000 to start and end, 20 per token of a tile (read-out), 300 + 40 a block for a cluster; the stream takes the
 //              longest of 210 per K block and block on an SM (alone: and a third per token), of 1800 per turn of the ring where
 //              a block has half the memory, of the weight at 6 TB/s and of the tiles at 14 TB/s
-//   pairs      3600 + 9.5 per column to start, read out and end; 110 + 0.95 per column per K block and round
+//   pairs      as pair_form
 // Clusters of five and seven are left out: seven blocks do not pack into a processing cluster of the chip (twice the time).
 struct Form {
     int tokens, split;                 // tokens 0: pairs
 };
-Form choose_form(const Product& q, int k_blocks, int sm_count) {
+Form choose_form(const Product& q, const PairForm& pairs, int k_blocks, int sm_count) {
     const int64_t kb = k_blocks;
-    const int columns = pair_columns(q, sm_count / 2);
-    const int64_t pair_tiles = (q.m + 255) / 256 * ((q.n + columns - 1) / columns), rounds = (pair_tiles + sm_count / 2 - 1) / (sm_count / 2);
-    int64_t least = 3600 + 95 * columns / 10 + rounds * kb * (2200 + 19 * columns) / 20;
+    int64_t least = pairs.time;
     Form best{0, 1};
     const int key = fpt::tuning_linear_tokens(), split_key = fpt::tuning_linear_split();
     if (key > 0) least = INT64_MAX;
@@ -1022,8 +1121,9 @@ int launch_product(const Product& q, LinearParams& p, const DeviceInfo& dev, cud
     p.m = int(q.m);
     p.n = int(q.n);
     p.k_blocks = int((q.k + kBlockK - 1) / kBlockK);
+    const PairForm pairs = pair_form(q, dev.sm_count);
     if constexpr (!A_MN) {
-        const Form form = choose_form(q, p.k_blocks, dev.sm_count);
+        const Form form = choose_form(q, pairs, p.k_blocks, dev.sm_count);
         switch (form.tokens) {
         case 16: return launch_split<DT, ACT, SLOPE, 16, B_MN>(q, p, dev, form.split, stream);
         case 32: return launch_split<DT, ACT, SLOPE, 32, B_MN>(q, p, dev, form.split, stream);
@@ -1032,7 +1132,7 @@ int launch_product(const Product& q, LinearParams& p, const DeviceInfo& dev, cud
         default: break;
         }
     }
-    return launch_pair<DT, ACT, SLOPE, A_MN, B_MN>(q, p, dev, stream);
+    return launch_pair<DT, ACT, SLOPE, A_MN, B_MN>(q, p, dev, pairs, stream);
 }
 
 bool aligned16(const void* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0; }

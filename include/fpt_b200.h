@@ -468,8 +468,8 @@ int fpt_selftest_bounded_wait(void* status, void* report, int64_t limit_ns, int 
  * tiles is even, 0 (default) one: measured slower (no accumulator left to alternate);
  * key "linear_tokens": fpt_linear and its products: 16, 32, 64 or 128 tokens per tile of the few-row form, 0 the form on
  * pairs of CTAs, -1 (default) by size; key "linear_split": blocks that share an output tile of the few-row form along K
- * (1..8), 0 (default) by size; key "linear_columns": columns of an output tile of the pair form (64..256, a multiple of
- * 32), 0 (default) by size;
+ * (1..8), with linear_tokens 0 pairs that share one (1, 2, 4), 0 (default) by size; key "linear_columns": columns of an
+ * output tile of the pair form (64..256, a multiple of 32), 0 (default) by size;
  * key "gate_up_tile_rows": rows per tile of the single-CTA forms, 128 or 256; 0 (default) = 256 for one group (both halves
  * of a tile share every weight tile: fewer bytes per product, which under the power cap is the faster form), 128 for
  * grouped problems (a ragged group wastes less of a smaller tile). */

@@ -141,6 +141,18 @@ def test_every_tile_width(cuda, tuning, columns):
     check_linear_status()
 
 
+@pytest.mark.parametrize("split, columns", [(2, 64), (2, 128), (2, 256), (4, 128), (4, 256)])
+def test_pairs_that_share_a_tile(cuda, tuning, split, columns):
+    """The K blocks of a tile over the pairs of a cluster, whole and ragged runs of them (the weight's gradient contracts over the
+    rows: fewer K blocks than pairs fall back to one)."""
+    for shape in ((300, 520, 264), (70, 1288, 1003), (513, 640, 40), (1100, 1024, 512)):
+        tuning(0, split, columns)
+        args = inputs(*shape, torch.bfloat16, cuda)
+        y = check(*args, "gelu", what=f"{shape}")
+        assert torch.equal(y, linear_act(*args[:4], activation="gelu"))
+    check_linear_status()
+
+
 def test_several_tiles_per_block(cuda, tuning):
     """More output tiles than pairs of SMs: the persistent form goes round and alternates its accumulators."""
     tuning(0)
