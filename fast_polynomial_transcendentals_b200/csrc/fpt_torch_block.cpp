@@ -232,6 +232,7 @@ struct QkRopeBackward : torch::autograd::Node {
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         no_second_gradient("qk_rope");
+        at::AutoDispatchBelowADInplaceOrView below;    // no keys of autograd on the way to the kernels
         variable_list out(4);
         for (int i = 0; i < 2; ++i)
             if (!grads[i].defined()) grads[i] = input_metadata(i).zeros_like();
@@ -471,6 +472,7 @@ struct LinearBackward : torch::autograd::Node {
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         no_second_gradient("linear_act");
+        at::AutoDispatchBelowADInplaceOrView below;
         variable_list result(4);
         if (!grads[0].defined()) return result;
         const bool want_x = task_should_compute_output(0), want_w = task_should_compute_output(1), want_b = has_bias && task_should_compute_output(2);
