@@ -18,8 +18,8 @@
 // once and walks over the heads with them.  The passes are bound by memory traffic, 2 (forward) or 3 (backward) values per
 // value of q and k, once instructions and shared-memory reads are few enough: pairs are kept as two fp32 vectors (first
 // members, second members), which costs nothing to unpack, and handled by the two-wide fp32 instructions.
-// Measured, 2 x 4096 tokens x (32 + 8) heads x 128 bf16: forward with the norm 29.2 us = 5.7 TB/s, backward 55 us = 4.6 TB/s
-// (bound by instruction issue at 16 warps an SM); rotation alone of 15840 such tokens 50.0 us = 6.5 TB/s.
+// Measured, 2 x 4096 tokens x (32 + 8) heads x 128 bf16: forward with the norm 29.2 us = 5.7 TB/s, backward 46 us = 5.4 TB/s
+// (next to the memory bound by latencies at 16 warps an SM); rotation alone of 15840 such tokens 50.0 us = 6.5 TB/s.
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -39,7 +39,7 @@ constexpr int kStages = 3;              // items of a thread in its ring
 constexpr int kBwdTrig = 512;           // tokens x pairs of a tile of the backward pass (two entries a thread, two tiles)
 // Blocks an SM holds, by registers (16-bit data; 2 in fp32).  Measured: the forward pass with the norm 29.5 us at 3 and 33.3 at 4
 // (which spills), the rotation alone 51.8 at 3 and 50.8 at 4, forward and backward pass together 121 with the backward
-// pass at 3 (spills) and 87 at 2.
+// pass at 3 (spills) and 87 at 2 (before the shares of share_blocks).
 template <class T, bool NORM>
 constexpr int kFwdBlocks = sizeof(T) == 4 ? 2 : NORM ? 3 : 4;
 constexpr int kBwdBlocks = 2;
@@ -912,13 +912,49 @@ extern "C" int fpt_qk_rope(void* q_out, void* k_out, const void* q, const void* 
 }
 
 namespace {
-// blocks of the backward pass on the query side and on the key side: as many as are resident, shared out by the heads; the
-// sines and cosines of a token cost about as much as one head
-void bwd_blocks(int64_t q_heads, int64_t k_heads, int sm_count, uint32_t (&blocks)[2]) {
-    const int64_t total = int64_t(sm_count) * kBwdBlocks;
-    const int64_t q = q_heads ? q_heads + 1 : 0, k = k_heads ? k_heads + 1 : 0;
-    blocks[0] = q ? uint32_t(std::max<int64_t>(1, (total * q + (q + k) / 2) / (q + k))) : 0u;
-    blocks[1] = k ? uint32_t(std::max<int64_t>(1, total - int64_t(blocks[0]))) : 0u;
+// Tiles of the backward pass and its blocks, as many as are resident, shared out between queries and keys.  A tile takes as many
+// steps as its groups have heads, and kTileCost more (sines, addresses, a barrier); the shares are those for which the side that
+// takes longest, in whole rounds of tiles, is done first.  Measured against shares by heads alone (a tile's own cost as one
+// head): 2 x 4096 tokens of 32 + 8 heads of 128 the backward pass 55 us and 46, 3063 tokens of 12 + 4 heads of 64 with the forward
+// pass 17.0 and 15.5, 8192 tokens of 8 + 1 heads of 256 53 and 35, of 40 + 8 heads of 80 58 and 62.  The constant: 0.5 .. 3 differ
+// by less than that.
+constexpr float kTileCost = 1.5f;
+void share_blocks(QkRopeArgs& a, uint32_t groups, int64_t seq, int sm_count) {
+    const uint32_t total = uint32_t(sm_count * kBwdBlocks);
+    float cost[2] = {0.0f, 0.0f};      // of a token, then of a tile
+    for (int s = 0; s < 2; ++s) {
+        Side& d = a.side[s];
+        if (!d.heads) continue;
+        d.tile_tokens = tile_tokens(groups, d.heads, a.pairs.d, 8, kBwdTrig);
+        cost[s] = float(d.heads) + kTileCost * float(groups) / float(d.tile_tokens);
+    }
+    for (int s = 0; s < 2; ++s) {
+        Side& d = a.side[s];
+        if (!d.heads) continue;
+        // no more tokens a tile than keep every block busy
+        const float blocks = float(total) * cost[s] / (cost[0] + cost[1]);
+        while (d.tile_tokens > 1 && float(a.tokens / d.tile_tokens) < blocks) d.tile_tokens /= 2;
+        if (!reach(d.xs, seq, d.heads, d.tile_tokens) || !reach(d.gs, seq, d.heads, d.tile_tokens)) d.tile_tokens = 1u;
+        d.tiles = (a.tokens + d.tile_tokens - 1) / d.tile_tokens;
+        d.blocks = std::min(total, d.tiles);
+    }
+    Side &q = a.side[0], &k = a.side[1];
+    if (!q.heads || !k.heads) return;
+    const auto steps = [&](const Side& d) { return float((d.heads + groups / d.tile_tokens - 1) / (groups / d.tile_tokens)) + kTileCost; };
+    const float q_tile = steps(q), k_tile = steps(k);
+    const float even = (float(q.tiles) * q_tile + float(k.tiles) * k_tile) / float(total);      // time with nothing left over
+    const uint32_t most = std::max(1u, uint32_t(even / q_tile));
+    float least = 1e30f;
+    for (uint32_t rounds = most > 2 ? most - 2 : 1; rounds < most + 6; ++rounds) {
+        const uint32_t blocks = (q.tiles + rounds - 1) / rounds;
+        if (blocks >= total) continue;
+        const float time = std::max(float(rounds) * q_tile, float((k.tiles + total - blocks - 1) / (total - blocks)) * k_tile);
+        if (time < least) {
+            least = time;
+            q.blocks = blocks;
+            k.blocks = std::min(total - blocks, k.tiles);
+        }
+    }
 }
 }  // namespace
 
@@ -926,9 +962,7 @@ extern "C" int64_t fpt_qk_norm_rope_bwd_workspace_bytes(int64_t q_heads, int64_t
     if (q_heads < 0 || k_heads < 0 || q_heads + k_heads == 0 || head_dim <= 0) return 0;
     DeviceInfo dev;
     if (current_device_info(&dev)) return 0;
-    uint32_t blocks[2];
-    bwd_blocks(q_heads, k_heads, dev.sm_count, blocks);
-    return (int64_t(blocks[0]) + blocks[1]) * head_dim * int64_t(sizeof(float));
+    return int64_t(dev.sm_count) * kBwdBlocks * head_dim * int64_t(sizeof(float));
 }
 
 extern "C" int fpt_qk_norm_rope_bwd(void* dq, void* dk, void* dq_weight, void* dk_weight, const void* dq_out, const void* dk_out,
@@ -958,27 +992,17 @@ extern "C" int fpt_qk_norm_rope_bwd(void* dq, void* dk, void* dq_weight, void* d
     DeviceInfo dev;
     if (int rc = current_device_info(&dev)) return rc;
     uint32_t blocks[2] = {0, 0};
-    if (a.tokens) bwd_blocks(q_heads, k_heads, dev.sm_count, blocks);
     if (weights && a.tokens) {
         if (!workspace) return FPT_ERR_NULL_POINTER;
-        if (workspace_bytes < (int64_t(blocks[0]) + blocks[1]) * head_dim * int64_t(sizeof(float))) return FPT_ERR_SCRATCH_TOO_SMALL;
+        if (workspace_bytes < int64_t(dev.sm_count) * kBwdBlocks * head_dim * int64_t(sizeof(float))) return FPT_ERR_SCRATCH_TOO_SMALL;
     }
     float* partial = static_cast<float*>(workspace);
     if (a.tokens) {
         a.eps = eps;
         a.sin_sign = 0x80000000u;
         const uint32_t groups = uint32_t(kThreads / group_lanes(a.units));
-        for (int s = 0; s < 2; ++s) {
-            Side& d = a.side[s];
-            if (!d.heads) continue;
-            d.tile_tokens = tile_tokens(groups, d.heads, uint32_t(pairs), 8, kBwdTrig);
-            // no more tokens a tile than keep every block busy
-            while (d.tile_tokens > 1 && a.tokens / d.tile_tokens < blocks[s]) d.tile_tokens /= 2;
-            if (!reach(d.xs, seq, d.heads, d.tile_tokens) || !reach(d.gs, seq, d.heads, d.tile_tokens)) d.tile_tokens = 1u;
-            d.tiles = (a.tokens + d.tile_tokens - 1) / d.tile_tokens;
-            blocks[s] = std::min(blocks[s], d.tiles);
-            d.blocks = blocks[s];
-        }
+        share_blocks(a, groups, seq, dev.sm_count);
+        for (int s = 0; s < 2; ++s) blocks[s] = a.side[s].heads ? a.side[s].blocks : 0u;
         for (int s = 0; s < 2; ++s)
             a.side[s].partial = (s ? dk_weight : dq_weight) ? partial + (s ? int64_t(blocks[0]) * head_dim : 0) : nullptr;
         const unsigned grid = blocks[0] + blocks[1];
