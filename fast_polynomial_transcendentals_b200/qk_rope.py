@@ -11,6 +11,9 @@ gradient) and take the same parameter, `sfu_repro.rope.rope_phase_increments`: 3
 phase `position * increment` wraps as the angle does, so it is exact at every 32- or 64-bit position.  All arithmetic here
 is fp32 with one rounding at the end, whatever the dtype (float16, bfloat16 or float32).
 
+Forward and backward pass can be captured into CUDA graphs; drop every eager graph of the same leaves before a backward pass is
+captured, as for PyTorch's own operators (a leaf's gradient accumulation stays on the stream of the graph that made it).
+
 A second derivative is refused (RuntimeError); so is a call whose shapes, dtypes or devices do not fit.
 """
 from __future__ import annotations

@@ -198,6 +198,45 @@ def test_adapter_leaves_hooked_projections_alone(cuda):
         assert torch.equal(model(x), want)
 
 
+def test_calls_from_two_threads_at_once(cuda):
+    """Two threads, each on a stream of its own, few and many rows, forward and gradients: the same bits as one after another."""
+    import threading
+    inc = rope_phase_increments(D, device=cuda)
+
+    def step(seed):
+        g = torch.Generator(device=cuda)
+        g.manual_seed(seed)
+        out = []
+        for rows in (3, 256, 700):
+            x = torch.randn(rows, 2048, device=cuda, generator=g).to(BF).requires_grad_()
+            w = (torch.randn(6 * D, 2048, device=cuda, generator=g) / 45).to(BF).requires_grad_()
+            y = linear_act(x, w, activation="gelu")
+            q, k = qk_rope.qk_norm_rope(*y.view(1, rows, 6, D).split([4, 2], dim=2), None, None, inc)
+            out += [y, q, k, *torch.autograd.grad((q, k), [x, w], [torch.ones_like(q), torch.ones_like(k)])]
+        return out
+
+    want = [step(seed) for seed in (1, 2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got[i].append(step(i + 1))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    for i in range(2):
+        assert len(got[i]) == 10
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))
+    check_linear_status()
+
+
 def test_offsets_past_31_bits(cuda):
     """Results of more than 2^31 elements, rows checked at both ends and in between.  One rounding to bf16 (eps / 2 = 2^-8 of
     the value: eight significant bits) and fp32 sums of 64 terms of size 64 / 8 in all (18 u S, S < 100: below 3e-4)."""

@@ -145,9 +145,9 @@ def test_every_tile_width(cuda, tuning, columns):
 def test_pairs_that_share_a_tile(cuda, tuning, split, columns):
     """The K blocks of a tile over the pairs of a cluster, whole and ragged runs of them (the weight's gradient contracts over the
     rows: fewer K blocks than pairs fall back to one)."""
-    for shape in ((300, 520, 264), (70, 1288, 1003), (513, 640, 40), (1100, 1024, 512)):
+    for shape, dtype in (((300, 520, 264), "bf16"), ((70, 1288, 1003), "bf16"), ((513, 640, 40), "fp16"), ((1100, 1024, 512), "fp16")):
         tuning(0, split, columns)
-        args = inputs(*shape, torch.bfloat16, cuda)
+        args = inputs(*shape, DTYPES[dtype], cuda)
         y = check(*args, "gelu", what=f"{shape}")
         assert torch.equal(y, linear_act(*args[:4], activation="gelu"))
     check_linear_status()
