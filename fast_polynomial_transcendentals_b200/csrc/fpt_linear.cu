@@ -22,7 +22,7 @@
 //                         per SM; the blocks of a cluster share an output tile along K and add their fp32 partial sums over
 //                         distributed shared memory, in rank order (no atomics, no workspace, one launch).  Bound by the
 //                         weight's bytes: 1 row of 4096 -> 14336 bf16 21.7 us = 5.4 TB/s, 48 rows of 14336 -> 4096 24.6 us.
-//   linear_grad_act_kernel  6 bytes a value: 4096 x 4096 bf16 21 us.
+//   linear_grad_act_kernel  6 bytes a value: 4096 x 4096 bf16 18.1 us = 5.6 TB/s, with the column sums 20.5.
 //
 // Rounding: the epilogue works on the fp32 accumulators and rounds once.  The slope act' is kept in fp16 also beside bf16
 // data: it lies in about [-0.13, 1.13], where fp16 has eight times the resolution of bf16 at the same size, so the backward
@@ -823,6 +823,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 constexpr int kActThreads = 256;
 constexpr int kActColumns = 256;       // columns a block covers: 32 lanes of 8
 constexpr int kActRowLanes = kActThreads / 32;
+constexpr int kActBlocks = 5;           // resident on an SM, at 48 registers (asked for of the compiler: 22.4 us instead of 20.5)
 
 struct GradActParams {
     const uint16_t* dy;
@@ -842,6 +843,7 @@ __global__ void __launch_bounds__(kActThreads) linear_grad_act_kernel(const Grad
     const int column = blockIdx.x * kActColumns + 8 * lane;
     const int row_end = min(p.rows, (int(blockIdx.y) + 1) * p.chunk_rows);
     const int live = min(8, p.out - column);                    // columns of this lane that exist
+    wait_for_inputs();
     float sum[8] = {};
     if (live > 0) {
 #pragma unroll 2
@@ -946,13 +948,13 @@ struct Product {
 
 // A launch that may begin while the kernel before it in the stream drains; `cluster` 0: the kernel's own attribute, or none.
 template <class... P, class... A>
-cudaError_t launch_early(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t stream, const A&... args) {
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t stream, const A&... args) {
     if (smem > 48 * 1024) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(grid);
+    config.gridDim = grid;
     config.blockDim = dim3(threads);
     config.dynamicSmemBytes = smem;
     config.stream = stream;
@@ -1263,11 +1265,12 @@ extern "C" int fpt_linear_grad_weight(void* dw, const void* dz, const void* x, i
 }
 
 namespace {
-// rows one block sums: some six blocks for each of 148 SMs (a constant: the size of the workspace does not ask for a device), at
-// least 32 rows each
+// rows one block sums, at least 32: as many blocks as 148 SMs hold at once (a constant: the size of the workspace does not ask for a
+// device).  Measured with the column sums, 4096 x 4096 and 2048 x 14336 bf16, us at 3, 4, 5 and 6 blocks an SM: 23.3, 20.8, 20.5, 25.0
+// and 39.4, 34.2, 31.8, 39.4 (the sixth is a second round).
 int grad_act_chunk(int64_t rows, int64_t out) {
     const int64_t column_blocks = (out + kActColumns - 1) / kActColumns;
-    const int64_t chunks = std::max<int64_t>(1, 148 * 6 / column_blocks);
+    const int64_t chunks = std::max<int64_t>(1, 148 * kActBlocks / column_blocks);
     return int(std::min<int64_t>(rows, std::max<int64_t>((rows + chunks - 1) / chunks, std::max<int64_t>(32, (rows + 65534) / 65535))));
 }
 }  // namespace
@@ -1311,9 +1314,7 @@ extern "C" int fpt_linear_grad_act(void* dz, void* dbias, const void* dy, const 
         p.vec_dy = aligned16(dy, dy_ld);
         chunks = int((rows + p.chunk_rows - 1) / p.chunk_rows);
         const dim3 grid(unsigned((out_features + kActColumns - 1) / kActColumns), unsigned(chunks));
-        if (dtype == FPT_BF16) linear_grad_act_kernel<kBf16><<<grid, kActThreads, 0, stream>>>(p);
-        else linear_grad_act_kernel<kFp16><<<grid, kActThreads, 0, stream>>>(p);
-        if (int rc = cuda_status(cudaGetLastError())) return rc;
+        if (int rc = cuda_status(launch_early(dtype == FPT_BF16 ? linear_grad_act_kernel<kBf16> : linear_grad_act_kernel<kFp16>, grid, kActThreads, 0, 0u, stream, p))) return rc;
     }
     if (dbias) {
         return cuda_status(launch_early(linear_bias_grad_kernel, unsigned((out_features + 31) / 32), 256u, 0, 0u, stream,
