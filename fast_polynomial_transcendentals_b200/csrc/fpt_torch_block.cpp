@@ -52,6 +52,12 @@ void no_second_gradient(const char* name) {
     TORCH_CHECK(!at::GradMode::is_enabled(), name, " has no second gradient: run its backward pass without create_graph");
 }
 
+// a tangent would be lost below the autograd keys
+template <class... T>
+void no_forward_gradient(const char* name, const T&... inputs) {
+    TORCH_CHECK(!(torch::autograd::isFwGradDefined(inputs) || ...), name, " has no forward-mode derivative");
+}
+
 // ---- fpt_qk_rope --------------------------------------------------------------------------------------------------
 
 // the axis of every pair: the sections after one another (order 0), or dealt out in turn until an axis has its share (1)
@@ -258,6 +264,7 @@ std::tuple<Tensor, Tensor> qk_rope_autograd(const Tensor& q, const Tensor& k, co
                                             const Tensor& increments, const OptTensor& positions, at::IntArrayRef sections,
                                             int64_t order, int64_t pairing, bool norm, double eps, bool inverse) {
     const Tensor qw = q_weight.value_or(Tensor()), kw = k_weight.value_or(Tensor());
+    no_forward_gradient("qk_rope", q, k, qw, kw);
     std::shared_ptr<QkRopeBackward> node;
     if (torch::autograd::compute_requires_grad(q, k, qw, kw)) {
         node = std::shared_ptr<QkRopeBackward>(new QkRopeBackward(), torch::autograd::deleteNode);
@@ -493,6 +500,7 @@ Tensor linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& b
                        int64_t degree, int64_t source) {
     static const auto with_slope = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::linear_act_slope", "").typed<decltype(linear_act_slope)>();
     const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
+    no_forward_gradient("linear_act", x, weight, b, r);
     std::shared_ptr<LinearBackward> node;
     bool keep_slope = false;            // no activation: the slope is 1; only the residual wants a gradient: nobody asks for it
     if (torch::autograd::compute_requires_grad(x, weight, b, r)) {

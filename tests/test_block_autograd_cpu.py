@@ -1,0 +1,43 @@
+"""CPU: what the operators around the attention answer to PyTorch's automatic differentiation, on meta tensors (shapes and
+graphs without values)."""
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from fast_polynomial_transcendentals_b200 import linear, qk_rope  # noqa: F401  (registers torch.ops.fpt_b200)
+
+GELU = 4
+
+
+def meta(*shape, grad=False):
+    return torch.empty(*shape, dtype=torch.bfloat16, device="meta", requires_grad=grad)
+
+
+def layer(x, weight, bias=None, residual=None):
+    return torch.ops.fpt_b200.linear_act(x, weight, bias, residual, GELU, 0, 0)
+
+
+def heads(q, k, q_weight=None, k_weight=None, norm=True):
+    inc = torch.empty(32, dtype=torch.int32, device="meta")
+    return torch.ops.fpt_b200.qk_rope(q, k, q_weight, k_weight, inc, None, [], 0, 0, norm, 1e-6, False)
+
+
+LAYER = (4, 16), (8, 16), (8,), (4, 8)
+HEADS = (2, 3, 4, 64), (2, 3, 2, 64), (64,), (64,)
+
+
+@pytest.mark.parametrize("call, shapes", [(layer, LAYER), (heads, HEADS)])
+@pytest.mark.parametrize("which", range(4))
+def test_forward_mode_is_refused(call, shapes, which):
+    """No tangent is dropped without a word, whichever input carries it."""
+    args = [meta(*s) for s in shapes]
+    with forward_ad.dual_level():
+        args[which] = forward_ad.make_dual(args[which], torch.empty_like(args[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            call(*args)
+
+
+def test_jvp_of_the_rotation_alone_is_refused():
+    q, k = meta(2, 3, 4, 64), meta(2, 3, 2, 64)
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda q: heads(q, k, norm=False)[0], (q,), (torch.empty_like(q),))
