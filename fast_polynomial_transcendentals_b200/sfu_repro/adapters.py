@@ -246,6 +246,10 @@ def _epilogue_activation(fn: Any) -> str | None:
     return {"geluactivation": "gelu", "siluactivation": "silu"}.get(type(fn).__name__.lower())
 
 
+def _epilogue_input(x: Any) -> bool:
+    return x.is_cuda and x.dtype in (torch.bfloat16, torch.float16)
+
+
 def _as_it_comes(*modules: Any) -> bool:
     """Whether calling these does what their class does: no hooks, and for projections nn.Linear's own forward (a subclass or an
     instance with another one computes something else)."""
@@ -262,8 +266,8 @@ def patch_mlp_epilogues(model: nn.Module, *, variant: str = "native", degree: in
     ...), an erf GELU or SiLU in an activation slot, and nothing else that could act in between (dropout only where its
     probability is zero, no parameters of the module's own); others with the two projections are left alone and reported through
     `skipped`.  variant "native" evaluates the activation in fp32, "polynomial" runs the packed program (degree 5 for GELU, 3
-    for SiLU by default).  Inputs that are not float16 or bfloat16 on the GPU, or whose width is no multiple of 8, and
-    projections with hooks or a forward of their own (adapters on top of them) take the module's own forward."""
+    for SiLU by default).  Calls with more arguments than the input, inputs that are not float16 or bfloat16 on the GPU, or
+    whose width is no multiple of 8, and projections with hooks or a forward of their own (adapters on top of them) take the module's own forward."""
     patched = 0
     for name, module in model.named_modules():
         pair = next((p for p in _MLP_PAIRS if all(isinstance(getattr(module, n, None), nn.Linear) for n in p)), None)
@@ -283,7 +287,7 @@ def patch_mlp_epilogues(model: nn.Module, *, variant: str = "native", degree: in
 
         def forward(self, x, *args, _up=pair[0], _down=pair[1], _slot=slot, _act=activation, _degree=chosen, **kwargs):
             up, down = getattr(self, _up), getattr(self, _down)
-            if not (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and up.weight.dtype == down.weight.dtype == x.dtype
+            if args or kwargs or not (_epilogue_input(x) and up.weight.dtype == down.weight.dtype == x.dtype
                     and up.weight.shape[1] % 8 == 0 and down.weight.shape[1] % 8 == 0
                     and _as_it_comes(up, down, getattr(self, _slot))) or torch.is_autocast_enabled("cuda"):
                 return self.__dict__[_ORIGINAL](x, *args, **kwargs)

@@ -1,4 +1,5 @@
 """CPU: which feed-forward modules the epilogue adapter takes, and that what it takes behaves as before off the GPU."""
+import pytest
 import torch
 from torch import nn
 
@@ -65,3 +66,24 @@ def test_hooks_and_forwards_of_the_projections_are_seen():
     assert adapters._as_it_comes(plain.fc1, plain.fc2, plain.activation_fn)
     for model in (hooked, scaled, bound):
         assert not adapters._as_it_comes(model.fc1, model.fc2, model.activation_fn)
+
+
+@pytest.fixture
+def as_on_the_gpu(monkeypatch):
+    """The adapter's own path on the CPU: it takes every input, and the layer is its plain form."""
+    def plain(x, weight, bias=None, *, activation="none", degree=0, coeff_source="current"):
+        return {"none": lambda z: z, "gelu": nn.functional.gelu, "silu": nn.functional.silu}[activation](nn.functional.linear(x, weight, bias))
+    monkeypatch.setattr(adapters, "_epilogue_input", lambda x: True)
+    monkeypatch.setattr(adapters, "linear_act", plain)
+
+
+def test_further_arguments_are_not_dropped(as_on_the_gpu):
+    class Optional(Mlp):
+        def forward(self, x, residual=None):
+            y = super().forward(x)
+            return y if residual is None else y + residual
+
+    model, x, r = Optional(), torch.randn(3, 16), torch.randn(3, 16)
+    want = model(x), model(x, r), model(x, residual=r)
+    assert adapters.patch_mlp_epilogues(model) == 1
+    assert all(torch.equal(a, b) for a, b in zip(want, (model(x), model(x, r), model(x, residual=r))))
