@@ -10,6 +10,7 @@ reference does.
 """
 from __future__ import annotations
 
+import copy
 from types import MethodType
 from typing import Any, Callable
 
@@ -257,16 +258,69 @@ def _as_it_comes(*modules: Any) -> bool:
                    or (isinstance(m, nn.Linear) and (type(m).forward is not nn.Linear.forward or "forward" in m.__dict__))) for m in modules)
 
 
+def _plain_values(module: nn.Module) -> list[tuple[str | None, str, Any]]:
+    """(child or None for the module itself, attribute, value): numbers and flags that the module keeps as plain attributes, and
+    the probabilities of its dropouts."""
+    return [(None, n, v) for n, v in vars(module).items() if n != "training" and isinstance(v, (bool, int, float, str))] + \
+        [(n, "p", m.p) for n, m in module.named_children() if isinstance(m, nn.Dropout)]
+
+
+def _as_they_were(module: nn.Module, values: list[tuple[str | None, str, Any]]) -> bool:
+    return all(getattr(module if child is None else getattr(module, child), name, None) == value for child, name, value in values)
+
+
+class _Step(nn.Module):
+    """Stands in for one step of a forward: takes the tensor it is given next, untouched, and hands out the one after it."""
+
+    def __init__(self, takes: torch.Tensor, gives: torch.Tensor):
+        super().__init__()
+        self.takes, self.gives, self.calls = takes, gives, 0
+
+    def forward(self, x, *args, **kwargs):
+        if x is not self.takes or x._version or args or kwargs:
+            raise RuntimeError("another input than the step before gave")
+        self.calls += 1
+        return self.gives
+
+
+def _other_than_two_layers(module: nn.Module, pair: tuple[str, str], slot: str) -> str | None:
+    """None where the module's own forward is down(act(up(x))) and nothing else, in training and in evaluation, else what was
+    seen.  The forward runs on a shallow copy whose three steps are stand-ins that know their tensors by identity: a residual,
+    a second activation, a dropout that drops, a scale, a chunk or an in-place step in between or behind gives another one."""
+    up, down = getattr(module, pair[0]), getattr(module, pair[1])
+    if up.out_features != down.in_features:
+        return f"{pair[0]} gives {up.out_features} features, {pair[1]} takes {down.in_features}"
+    own = module.__dict__.get(_ORIGINAL, module.forward)
+    if getattr(own, "__func__", None) is not type(module).forward:
+        return "a forward of its own"
+    for training in (True, False):
+        x, hidden, active, y = (torch.zeros(2, 3, n) for n in (up.in_features, up.out_features, down.in_features, down.out_features))
+        steps = {pair[0]: _Step(x, hidden), slot: _Step(hidden, active), pair[1]: _Step(active, y)}
+        probe = copy.copy(module)
+        probe.__dict__["_modules"] = {**module._modules, **{n: s for n, s in steps.items() if n in module._modules}}
+        probe.__dict__.update({n: s for n, s in steps.items() if n not in module._modules})
+        probe.__dict__["training"] = training
+        try:
+            with torch.no_grad(), torch.random.fork_rng(devices=[]):
+                result = type(module).forward(probe, x)
+        except Exception as error:
+            return f"its forward is not down(act(up(x))): {type(error).__name__}: {error}"
+        if result is not y or y._version or any(s.calls != 1 for s in steps.values()):
+            return "its forward is not down(act(up(x)))"
+    return None
+
+
 def patch_mlp_epilogues(model: nn.Module, *, variant: str = "native", degree: int | None = None, coeff_source: str = "current",
                         skipped: list[tuple[str, str]] | None = None) -> int:
     """down(act(up(x))) as two kernels, bias and activation in the first one's epilogue and the bias in the second's
     (`linear.linear_act`), forward and backward; weights untouched, `restore` undoes it.
 
-    A module qualifies by structure: two `nn.Linear` under the usual names (`fc1 / fc2`, `up_proj / down_proj` without a gate,
-    ...), an erf GELU or SiLU in an activation slot, and nothing else that could act in between (dropout only where its
-    probability is zero, no parameters of the module's own); others with the two projections are left alone and reported through
-    `skipped`.  variant "native" evaluates the activation in fp32, "polynomial" runs the packed program (degree 5 for GELU, 3
-    for SiLU by default).  Calls with more arguments than the input, inputs that are not float16 or bfloat16 on the GPU, or
+    A module qualifies by structure, two `nn.Linear` under the usual names (`fc1 / fc2`, `up_proj / down_proj` without a gate,
+    ...), an erf GELU or SiLU in an activation slot and no parameters of its own, and by what its forward does: it is run once with
+    stand-ins for the three steps, and anything between or behind them (a residual, a dropout that drops, a second activation)
+    leaves it alone; such modules are reported through `skipped`.  variant "native" evaluates the activation in fp32, "polynomial" runs the packed program (degree 5 for GELU, 3
+    for SiLU by default).  Calls with more arguments than the input, modules whose plain attributes (a dropout probability) have
+    changed since, inputs that are not float16 or bfloat16 on the GPU, or
     whose width is no multiple of 8, and projections with hooks or a forward of their own (adapters on top of them) take the module's own forward."""
     patched = 0
     for name, module in model.named_modules():
@@ -283,11 +337,17 @@ def patch_mlp_epilogues(model: nn.Module, *, variant: str = "native", degree: in
                 skipped.append((name, f"also holds {', '.join(others)}" if others else
                                 f"{slot}={type(getattr(module, slot)).__name__}" if slot else "no activation slot"))
             continue
+        other = _other_than_two_layers(module, pair, slot)
+        if other is not None:
+            if skipped is not None:
+                skipped.append((name, other))
+            continue
         chosen = 0 if variant == "native" else degree if degree is not None else {"gelu": 5, "silu": 3}[activation]
 
-        def forward(self, x, *args, _up=pair[0], _down=pair[1], _slot=slot, _act=activation, _degree=chosen, **kwargs):
+        def forward(self, x, *args, _up=pair[0], _down=pair[1], _slot=slot, _act=activation, _degree=chosen,
+                    _plain=_plain_values(module), **kwargs):
             up, down = getattr(self, _up), getattr(self, _down)
-            if args or kwargs or not (_epilogue_input(x) and up.weight.dtype == down.weight.dtype == x.dtype
+            if args or kwargs or not _as_they_were(self, _plain) or not (_epilogue_input(x) and up.weight.dtype == down.weight.dtype == x.dtype
                     and up.weight.shape[1] % 8 == 0 and down.weight.shape[1] % 8 == 0
                     and _as_it_comes(up, down, getattr(self, _slot))) or torch.is_autocast_enabled("cuda"):
                 return self.__dict__[_ORIGINAL](x, *args, **kwargs)

@@ -87,3 +87,96 @@ def test_further_arguments_are_not_dropped(as_on_the_gpu):
     want = model(x), model(x, r), model(x, residual=r)
     assert adapters.patch_mlp_epilogues(model) == 1
     assert all(torch.equal(a, b) for a, b in zip(want, (model(x), model(x, r), model(x, residual=r))))
+
+
+class WithResidual(Mlp):
+    def forward(self, x, residual):
+        return super().forward(x) + residual
+
+
+class AddsItsInput(Mlp):
+    def forward(self, x):
+        y = super().forward(x)
+        y += x
+        return y
+
+
+class ActivatesTwice(Mlp):
+    def forward(self, x):
+        return self.activation_fn(super().forward(x))
+
+
+class DropsBetween(Mlp):
+    def __init__(self, p=0.1):
+        super().__init__()
+        self.p = p
+
+    def forward(self, x):
+        hidden = nn.functional.dropout(self.activation_fn(self.fc1(x)), p=self.p, training=self.training)
+        return self.fc2(hidden)
+
+
+class DropsInPlace(DropsBetween):
+    def forward(self, x):
+        y = self.fc2(self.activation_fn(self.fc1(x)))
+        return nn.functional.dropout(y, p=self.p, training=self.training, inplace=True)
+
+
+class GatedInside(Mlp):
+    def __init__(self):
+        super().__init__()
+        self.fc1 = nn.Linear(16, 64)
+
+    def forward(self, x):
+        hidden, gate = self.fc1(x).chunk(2, dim=-1)
+        return self.fc2(self.activation_fn(gate) * hidden)
+
+
+class GatedByItself(Mlp):
+    def forward(self, x):
+        hidden = self.fc1(x)
+        return self.fc2(self.activation_fn(hidden) * hidden)
+
+
+class SkipsItsActivation(Mlp):
+    def forward(self, x):
+        return self.fc2(self.fc1(x))
+
+
+class WithABias(Mlp):
+    def forward(self, x):
+        return super().forward(x), self.fc2.bias
+
+
+class ByItsWeights(Mlp):
+    def forward(self, x):
+        return self.fc2(self.activation_fn(nn.functional.linear(x, 2 * self.fc1.weight, self.fc1.bias)))
+
+
+@pytest.mark.parametrize("kind", [WithResidual, AddsItsInput, ActivatesTwice, DropsBetween, DropsInPlace, GatedInside, GatedByItself,
+                                  SkipsItsActivation, WithABias, ByItsWeights])
+def test_forwards_that_do_more_are_left_alone(kind):
+    model, skipped = kind(), []
+    state = torch.random.get_rng_state()
+    assert adapters.patch_mlp_epilogues(model, skipped=skipped) == 0 and [n for n, _ in skipped] == [""]
+    assert "forward" not in model.__dict__ and model.training and isinstance(model.fc1, nn.Linear)
+    assert torch.equal(state, torch.random.get_rng_state())
+
+
+def test_a_forward_set_on_the_module_is_left_alone():
+    model, skipped = Mlp(), []
+    model.forward = lambda x: 2 * x
+    assert adapters.patch_mlp_epilogues(model, skipped=skipped) == 0 and skipped == [("", "a forward of its own")]
+
+
+def test_a_dropout_that_begins_to_drop_is_not_lost(as_on_the_gpu):
+    for model, change in ((DropsBetween(0.0), lambda m: setattr(m, "p", 0.9)), (Mlp(dropout=0.0), lambda m: setattr(m.dropout, "p", 0.9))):
+        calls = []
+        assert adapters.patch_mlp_epilogues(model) == 1
+        original = model.__dict__[adapters._ORIGINAL]
+        model.__dict__[adapters._ORIGINAL] = lambda x: calls.append(1) or original(x)
+        model(torch.randn(3, 16))
+        assert not calls                        # the fused path
+        change(model)
+        model(torch.randn(3, 16))
+        assert calls == [1]
