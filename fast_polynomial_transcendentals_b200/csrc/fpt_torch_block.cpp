@@ -238,20 +238,24 @@ struct QkRopeBackward : torch::autograd::Node {
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         no_second_gradient("qk_rope");
-        at::AutoDispatchBelowADInplaceOrView below;    // no keys of autograd on the way to the kernels
         variable_list out(4);
         for (int i = 0; i < 2; ++i)
             if (!grads[i].defined()) grads[i] = input_metadata(i).zeros_like();
+        // Everything is unpacked before the guard: a hook on a saved tensor (activation checkpointing) may run the forward pass
+        // again, with its own graph.
         const OptTensor pos = has_positions ? OptTensor(positions.unpack()) : OptTensor();
         const Tensor inc = increments.unpack();
         if (!norm) {                    // the rotation alone needs neither q nor k again
+            at::AutoDispatchBelowADInplaceOrView below;    // no keys of autograd on the way to the kernels
             std::tie(out[0], out[1]) = call_qk_rope(grads[0], grads[1], {}, {}, inc, pos, sections, order, pairing, false, 0.0, !inverse);
             return out;
         }
+        const Tensor q_in = q.unpack(), k_in = k.unpack();
+        const OptTensor qw = has_q_weight ? OptTensor(q_weight.unpack()) : OptTensor(), kw = has_k_weight ? OptTensor(k_weight.unpack()) : OptTensor();
         static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::qk_norm_rope_bwd", "").typed<decltype(qk_norm_rope_bwd)>();
         const bool dqw = has_q_weight && task_should_compute_output(2), dkw = has_k_weight && task_should_compute_output(3);
-        auto d = op.call(grads[0], grads[1], q.unpack(), k.unpack(), has_q_weight ? OptTensor(q_weight.unpack()) : OptTensor(),
-                         has_k_weight ? OptTensor(k_weight.unpack()) : OptTensor(), inc, pos, sections, order, pairing, eps, dqw, dkw);
+        at::AutoDispatchBelowADInplaceOrView below;
+        auto d = op.call(grads[0], grads[1], q_in, k_in, qw, kw, inc, pos, sections, order, pairing, eps, dqw, dkw);
         out[0] = std::get<0>(d);
         out[1] = std::get<1>(d);
         if (dqw) out[2] = std::get<2>(d);
@@ -479,14 +483,16 @@ struct LinearBackward : torch::autograd::Node {
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         no_second_gradient("linear_act");
-        at::AutoDispatchBelowADInplaceOrView below;
         variable_list result(4);
         if (!grads[0].defined()) return result;
         const bool want_x = task_should_compute_output(0), want_w = task_should_compute_output(1), want_b = has_bias && task_should_compute_output(2);
         if (want_x || want_w || want_b) {
             static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::linear_act_bwd", "").typed<decltype(linear_act_bwd)>();
-            auto d = op.call(grads[0], slope.unpack(), want_w ? OptTensor(x.unpack()) : OptTensor(), want_x ? OptTensor(weight.unpack()) : OptTensor(),
-                             shape, out, bias_dtype, want_x, want_w, want_b);
+            // unpacked before the guard, as above
+            const Tensor kept = slope.unpack();
+            const OptTensor x_in = want_w ? OptTensor(x.unpack()) : OptTensor(), weight_in = want_x ? OptTensor(weight.unpack()) : OptTensor();
+            at::AutoDispatchBelowADInplaceOrView below;
+            auto d = op.call(grads[0], kept, x_in, weight_in, shape, out, bias_dtype, want_x, want_w, want_b);
             if (want_x) result[0] = std::get<0>(d);
             if (want_w) result[1] = std::get<1>(d);
             if (want_b) result[2] = std::get<2>(d);

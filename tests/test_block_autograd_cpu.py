@@ -41,3 +41,30 @@ def test_jvp_of_the_rotation_alone_is_refused():
     q, k = meta(2, 3, 4, 64), meta(2, 3, 2, 64)
     with pytest.raises(RuntimeError, match="forward-mode"):
         torch.func.jvp(lambda q: heads(q, k, norm=False)[0], (q,), (torch.empty_like(q),))
+
+
+def checkpointed_layer(x, w, b, r):
+    return layer(x, w, b, r)
+
+
+def checkpointed_norm_of_the_layer(x, w, b, r):
+    return heads(layer(x, w, b, r).view(1, 4, 2, 64), layer(x, w).view(1, 4, 2, 64))[0].reshape(4, 128)
+
+
+def checkpointed_rotation(x, w, b, r):
+    return heads(layer(x, w, b, r).view(1, 4, 2, 64), x.view(1, 4, 2, 64), norm=False)[0].reshape(4, 128)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+@pytest.mark.parametrize("region", [checkpointed_layer, checkpointed_norm_of_the_layer, checkpointed_rotation])
+def test_checkpointed_regions(region, reentrant):
+    """A region that ends in one of the operators: its node is the first to need its saved tensors, and the region runs again
+    inside the node's unpacking."""
+    from torch.utils.checkpoint import checkpoint
+    args = [meta(4, 128, grad=True), meta(128, 128, grad=True), meta(128, grad=True), meta(4, 128, grad=True)]
+    for call in (lambda *a: checkpoint(region, *a, use_reentrant=reentrant),
+                 lambda *a: a[0] + checkpoint(region, *(2 * t for t in a), use_reentrant=reentrant)):
+        for t in args:
+            t.grad = None
+        call(*args).sum().backward()
+        assert all(t.grad is not None and t.grad.shape == t.shape for t in args)

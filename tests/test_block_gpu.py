@@ -261,3 +261,40 @@ def test_offsets_past_31_bits(cuda):
         one = qk_rope.rope_axes(q[b:b + 1, s:s + 1].contiguous(), k[b:b + 1, s:s + 1].contiguous(), inc,
                                 torch.tensor([[s]], device=cuda), [64], pairing="halves")
         assert torch.equal(got[0][b, s], one[0][0, 0]) and torch.equal(got[1][b, s], one[1][0, 0]), (b, s)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_checkpointed_block(cuda, reentrant):
+    """Activation checkpointing of the run, which ends in a layer with a residual: the same values, and gradients whose bits are the
+    same where they do not pass through the attention (it adds its dQ in no fixed order: root mean square below 2^-8)."""
+    from torch.utils.checkpoint import checkpoint
+    w, x, inc, positions, sections = case(cuda, False)
+    leaves = {n: t.detach().requires_grad_() for n, t in w.items()}
+    xs, grad = x.detach().requires_grad_(), torch.randn_like(x)
+    runs = []
+    for call in (block, lambda *args: checkpoint(block, *args, use_reentrant=reentrant)):
+        for t in (xs, *leaves.values()):
+            t.grad = None
+        y = call(xs, leaves, inc, positions, sections)
+        y.backward(grad)
+        runs.append((y.detach(), {"x": xs.grad, **{n: t.grad for n, t in leaves.items()}}))
+    assert torch.equal(runs[0][0], runs[1][0])
+    for n, want in runs[0][1].items():
+        got = runs[1][1][n]
+        if n in ("up", "up_bias", "down", "down_bias"):
+            assert torch.equal(got, want), n
+        else:
+            assert ((got.float() - want.float()).norm() / want.float().norm()).item() < 2.0 ** -8, n
+    fa4.check_attention_status()
+    check_linear_status()
+
+
+def test_a_checkpointed_patched_feed_forward(cuda):
+    from torch.utils.checkpoint import checkpoint
+    model = Mlp(nn.GELU()).to(cuda, BF)
+    assert adapters.patch_mlp_epilogues(model) == 1
+    x = torch.randn(40, 256, device=cuda).to(BF).requires_grad_()
+    want = torch.autograd.grad(x + model(x), [x, *model.parameters()], torch.ones_like(x))
+    y = x + checkpoint(model, x, use_reentrant=False)
+    got = torch.autograd.grad(y, [x, *model.parameters()], torch.ones_like(x))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
