@@ -469,10 +469,15 @@ Tensor call_linear(const Tensor& x, const Tensor& weight, const OptTensor& bias,
     return op.call(x, weight, bias, residual, function, degree, source);
 }
 
+// linear_act_bwd as the dispatcher knows it: sizes may be symbols of a compiled graph
+using linear_act_bwd_symbolic = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&,
+                                                                   c10::SymIntArrayRef, c10::SymInt, int64_t, bool, bool, bool);
+
 struct LinearBackward : torch::autograd::Node {
     SavedVariable x, weight, slope;
-    std::vector<int64_t> shape;         // of x
-    int64_t out = 0, bias_dtype = 0;
+    std::vector<c10::SymInt> shape;     // of x
+    c10::SymInt out = 0;
+    int64_t bias_dtype = 0;
     bool has_bias = false;
 
     std::string name() const override { return "LinearActBackward"; }
@@ -487,7 +492,7 @@ struct LinearBackward : torch::autograd::Node {
         if (!grads[0].defined()) return result;
         const bool want_x = task_should_compute_output(0), want_w = task_should_compute_output(1), want_b = has_bias && task_should_compute_output(2);
         if (want_x || want_w || want_b) {
-            static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::linear_act_bwd", "").typed<decltype(linear_act_bwd)>();
+            static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::linear_act_bwd", "").typed<linear_act_bwd_symbolic>();
             // unpacked before the guard, as above
             const Tensor kept = slope.unpack();
             const OptTensor x_in = want_w ? OptTensor(x.unpack()) : OptTensor(), weight_in = want_x ? OptTensor(weight.unpack()) : OptTensor();
@@ -514,8 +519,8 @@ Tensor linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& b
         node->set_next_edges(torch::autograd::collect_next_edges(x, weight, b, r));
         if (weight.requires_grad()) node->x = SavedVariable(x, false);
         if (x.requires_grad()) node->weight = SavedVariable(weight, false);
-        node->shape = x.sizes().vec();
-        node->out = weight.dim() ? weight.size(0) : 0;
+        node->shape = x.sym_sizes().vec();
+        node->out = weight.dim() ? weight.sym_size(0) : c10::SymInt(0);
         node->has_bias = b.defined();
         node->bias_dtype = b.defined() ? dtype_id(b.scalar_type()) : FPT_FP32;
         keep_slope = function != FPT_FN_NONE && (x.requires_grad() || weight.requires_grad() || (b.defined() && b.requires_grad()));
@@ -558,7 +563,7 @@ TORCH_LIBRARY_FRAGMENT(fpt_b200, m) {
           "bool want_q_weight, bool want_k_weight) -> (Tensor, Tensor, Tensor, Tensor)");
     m.def("linear_act(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int function, int degree, int source) -> Tensor");
     m.def("linear_act_slope(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int function, int degree, int source) -> (Tensor, Tensor)");
-    m.def("linear_act_bwd(Tensor dy, Tensor slope, Tensor? x, Tensor? weight, int[] x_shape, int out, int bias_dtype, bool want_x, "
+    m.def("linear_act_bwd(Tensor dy, Tensor slope, Tensor? x, Tensor? weight, SymInt[] x_shape, SymInt out, int bias_dtype, bool want_x, "
           "bool want_weight, bool want_bias) -> (Tensor, Tensor, Tensor)");
 }
 

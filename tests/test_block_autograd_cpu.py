@@ -68,3 +68,88 @@ def test_checkpointed_regions(region, reentrant):
             t.grad = None
         call(*args).sum().backward()
         assert all(t.grad is not None and t.grad.shape == t.shape for t in args)
+
+
+@pytest.fixture
+def cpu_kernels():
+    """Plain forms of the kernels behind the dispatcher's CPU key (GELU and the norm with adjacent pairs and no angle), for what
+    autograd and the compiler do above them."""
+    def z_of(x, weight, bias):
+        z = x.double() @ weight.double().T
+        return z if bias is None else z + bias.double()
+
+    def forward(x, weight, bias, residual, function, degree, source):
+        y = torch.nn.functional.gelu(z_of(x, weight, bias))
+        return (y if residual is None else y + residual.double()).to(x.dtype)
+
+    def with_slope(x, weight, bias, residual, function, degree, source):
+        z = z_of(x, weight, bias).reshape(-1, weight.shape[0])
+        slope = torch.special.ndtr(z) + z * torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
+        kept = torch.zeros(z.shape[0], (z.shape[1] + 7) // 8 * 8, dtype=torch.float16)
+        kept[:, :z.shape[1]] = slope
+        return forward(x, weight, bias, residual, function, degree, source), kept
+
+    def backward(dy, slope, x, weight, x_shape, out, bias_dtype, want_x, want_weight, want_bias):
+        dz = dy.reshape(-1, out).double() * slope[:, :out].double()
+        none = dy.new_empty(0)
+        return ((dz @ weight.double()).to(dy.dtype).reshape(x_shape) if want_x else none,
+                (dz.T @ x.double().reshape(-1, x_shape[-1])).to(dy.dtype) if want_weight else none,
+                dz.sum(0).to((torch.float16, torch.bfloat16, torch.float32)[bias_dtype]) if want_bias else none)
+
+    def norm(t, w):
+        u = t.double() * torch.rsqrt(t.double().square().mean(-1, keepdim=True) + 1e-6)
+        return (u if w is None else u * w.double()).to(t.dtype)
+
+    def rope(q, k, q_weight, k_weight, inc, positions, sections, order, pairing, with_norm, eps, inverse):
+        return (norm(q, q_weight), norm(k, k_weight)) if with_norm else (q.clone(), k.clone())
+
+    def rope_backward(dq, dk, q, k, q_weight, k_weight, inc, positions, sections, order, pairing, eps, want_q, want_k):
+        out = []
+        for g, t, w, want in ((dq, q, q_weight, want_q), (dk, k, k_weight, want_k)):
+            t, g = t.double(), g.double()
+            r = torch.rsqrt(t.square().mean(-1, keepdim=True) + 1e-6)
+            u, h = t * r, g if w is None else g * w.double()
+            out.append(((r * (h - u * (h * u).mean(-1, keepdim=True))).to(dq.dtype), (g * u).sum((0, 1, 2)).to(w.dtype) if want else q.new_empty(0)))
+        return out[0][0], out[1][0], out[0][1], out[1][1]
+
+    library = torch.library.Library("fpt_b200", "IMPL")
+    for name, kernel in (("linear_act", forward), ("linear_act_slope", with_slope), ("linear_act_bwd", backward), ("qk_rope", rope),
+                         ("qk_norm_rope_bwd", rope_backward)):
+        library.impl(name, kernel, "CPU")
+    yield
+    library._destroy()
+
+
+def values(*shape, seed=0, grad=True):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16).requires_grad_(grad)
+
+
+def layer_args(rows):
+    return [values(rows, 16, seed=1), values(24, 16, seed=2), values(24, seed=3), values(rows, 24, seed=4)]
+
+
+def heads_args(rows):
+    return [values(2, rows, 4, 64, seed=1), values(2, rows, 2, 64, seed=2), values(64, seed=3), values(64, seed=4)]
+
+
+def cpu_heads(q, k, q_weight, k_weight):
+    return torch.cat(torch.ops.fpt_b200.qk_rope(q, k, q_weight, k_weight, torch.zeros(32, dtype=torch.int32), None, [], 0, 0, True, 1e-6, False), dim=2)
+
+
+@pytest.mark.parametrize("call, make, row_axis", [(layer, layer_args, 0), (cpu_heads, heads_args, 1)], ids=["layer", "heads"])
+@pytest.mark.parametrize("marked", [True, False])
+def test_compiled_training_step_with_any_number_of_rows(cpu_kernels, call, make, row_axis, marked):
+    """One graph for all row counts: none is written into the operators' gradients."""
+    torch._dynamo.reset()
+    compiled = torch.compile(call, backend="aot_eager", fullgraph=True, dynamic=None if marked else True)
+    with torch._dynamo.config.patch(recompile_limit=2, error_on_recompile=False):
+        for rows in (50, 3, 7, 11, 200):
+            args = make(rows)
+            if marked:
+                for t in args:
+                    if t.dim() > row_axis and t.shape[row_axis] == rows and t.dim() > 1:
+                        torch._dynamo.mark_dynamic(t, row_axis)
+            want = torch.autograd.grad(call(*args).float().sum(), args)
+            got = torch.autograd.grad(compiled(*args).float().sum(), args)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), rows
+    torch._dynamo.reset()

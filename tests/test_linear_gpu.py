@@ -384,3 +384,20 @@ def test_random_shapes(cuda):
     for i in range(24):
         rows, dim, out = (int(torch.randint(lo, hi, (1,), generator=g)) for lo, hi in ((1, 700), (1, 60), (1, 900)))
         check(*inputs(rows, 8 * dim, out, DTYPES["fp16" if i % 3 == 0 else "bf16"], cuda, seed=i), ACTIVATIONS[i % 5], what=str((rows, 8 * dim, out)))
+
+
+def test_compiled_training_step_with_any_number_of_rows(cuda):
+    """One compiled graph, row counts of every tile form: the bits of the eager call."""
+    torch._dynamo.reset()
+    f = lambda x, w, b, r: linear_act(x, w, b, r, activation="gelu") * 2
+    compiled = torch.compile(f, backend="aot_eager", fullgraph=True)
+    with torch._dynamo.config.patch(recompile_limit=2):
+        for rows in (12, 2, 40, 300, 1025):
+            x, w, b, r, dy = inputs(rows, 64, 40, torch.bfloat16, cuda, seed=rows)
+            leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+            for t in (leaves[0], leaves[3]):
+                torch._dynamo.mark_dynamic(t, 0)
+            want = torch.autograd.grad(f(*leaves), leaves, dy)
+            got = torch.autograd.grad(compiled(*leaves), leaves, dy)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), rows
+    torch._dynamo.reset()
