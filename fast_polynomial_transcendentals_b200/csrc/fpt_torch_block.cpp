@@ -48,9 +48,41 @@ bool floating(const Tensor& x) {
     return x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat;
 }
 
-void no_second_gradient(const char* name) {
-    TORCH_CHECK(!at::GradMode::is_enabled(), name, " has no second gradient: run its backward pass without create_graph");
+// Gradients are not themselves differentiable.  Where autograd records the backward pass (create_graph) it is refused.  The
+// transforms of torch.func always record it, also for a first derivative: there the gradients come back with a node that
+// refuses when a second derivative reaches it.
+[[noreturn]] void no_second_gradient(const char* name) {
+    TORCH_CHECK(false, name, " has no second gradient: run its backward pass without create_graph");
 }
+bool of_transform(const Tensor& t) { return t.defined() && t.key_set().has(c10::DispatchKey::FuncTorchGradWrapper); }
+// whether a transform records this backward pass
+template <class... T>
+bool in_transform(const char* name, const T&... tensors) {
+    if (!at::GradMode::is_enabled()) return false;
+    if (!c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode) && !(of_transform(tensors) || ...))
+        no_second_gradient(name);
+    return true;
+}
+struct NoSecondGradient : torch::autograd::Node {
+    const char* operator_name;
+    explicit NoSecondGradient(const char* of) : operator_name(of) {}
+    std::string name() const override { return "NoSecondGradient"; }
+    torch::autograd::variable_list apply(torch::autograd::variable_list&&) override { no_second_gradient(operator_name); }
+};
+template <class... T>
+void refuse_to_go_on(const char* name, std::initializer_list<Tensor> results, const T&... of) {
+    if (!torch::autograd::compute_requires_grad(of...)) return;
+    std::shared_ptr<NoSecondGradient> node(new NoSecondGradient(name), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(of...));
+    for (const Tensor& t : results) torch::autograd::set_history(t, node);
+}
+// No keys of autograd on the way to the kernels, which spares host time, unless the backward pass is itself recorded.
+struct BelowAutograd {
+    std::optional<at::AutoDispatchBelowADInplaceOrView> guard;
+    explicit BelowAutograd(bool recorded) {
+        if (!recorded) guard.emplace();
+    }
+};
 
 // a tangent would be lost below the autograd keys
 template <class... T>
@@ -237,7 +269,6 @@ struct QkRopeBackward : torch::autograd::Node {
     }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
-        no_second_gradient("qk_rope");
         variable_list out(4);
         for (int i = 0; i < 2; ++i)
             if (!grads[i].defined()) grads[i] = input_metadata(i).zeros_like();
@@ -246,7 +277,7 @@ struct QkRopeBackward : torch::autograd::Node {
         const OptTensor pos = has_positions ? OptTensor(positions.unpack()) : OptTensor();
         const Tensor inc = increments.unpack();
         if (!norm) {                    // the rotation alone needs neither q nor k again
-            at::AutoDispatchBelowADInplaceOrView below;    // no keys of autograd on the way to the kernels
+            const BelowAutograd below(at::GradMode::is_enabled());      // linear: its gradient has one
             std::tie(out[0], out[1]) = call_qk_rope(grads[0], grads[1], {}, {}, inc, pos, sections, order, pairing, false, 0.0, !inverse);
             return out;
         }
@@ -254,7 +285,7 @@ struct QkRopeBackward : torch::autograd::Node {
         const OptTensor qw = has_q_weight ? OptTensor(q_weight.unpack()) : OptTensor(), kw = has_k_weight ? OptTensor(k_weight.unpack()) : OptTensor();
         static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::qk_norm_rope_bwd", "").typed<decltype(qk_norm_rope_bwd)>();
         const bool dqw = has_q_weight && task_should_compute_output(2), dkw = has_k_weight && task_should_compute_output(3);
-        at::AutoDispatchBelowADInplaceOrView below;
+        const BelowAutograd below(in_transform("qk_rope", grads[0], grads[1], q_in, k_in, qw.value_or(Tensor()), kw.value_or(Tensor())));
         auto d = op.call(grads[0], grads[1], q_in, k_in, qw, kw, inc, pos, sections, order, pairing, eps, dqw, dkw);
         out[0] = std::get<0>(d);
         out[1] = std::get<1>(d);
@@ -263,6 +294,22 @@ struct QkRopeBackward : torch::autograd::Node {
         return out;
     }
 };
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rope_bwd_autograd(const Tensor& dq_out, const Tensor& dk_out, const Tensor& q, const Tensor& k,
+                                                                     const OptTensor& q_weight, const OptTensor& k_weight, const Tensor& increments,
+                                                                     const OptTensor& positions, at::IntArrayRef sections, int64_t order,
+                                                                     int64_t pairing, double eps, bool want_q_weight, bool want_k_weight) {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::qk_norm_rope_bwd", "").typed<decltype(qk_norm_rope_bwd)>();
+    const Tensor qw = q_weight.value_or(Tensor()), kw = k_weight.value_or(Tensor());
+    no_forward_gradient("qk_norm_rope_bwd", dq_out, dk_out, q, k, qw, kw);
+    std::tuple<Tensor, Tensor, Tensor, Tensor> d;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        d = op.call(dq_out, dk_out, q, k, q_weight, k_weight, increments, positions, sections, order, pairing, eps, want_q_weight, want_k_weight);
+    }
+    refuse_to_go_on("qk_rope", {std::get<0>(d), std::get<1>(d), std::get<2>(d), std::get<3>(d)}, dq_out, dk_out, q, k, qw, kw);
+    return d;
+}
 
 std::tuple<Tensor, Tensor> qk_rope_autograd(const Tensor& q, const Tensor& k, const OptTensor& q_weight, const OptTensor& k_weight,
                                             const Tensor& increments, const OptTensor& positions, at::IntArrayRef sections,
@@ -487,17 +534,16 @@ struct LinearBackward : torch::autograd::Node {
     }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
-        no_second_gradient("linear_act");
         variable_list result(4);
         if (!grads[0].defined()) return result;
         const bool want_x = task_should_compute_output(0), want_w = task_should_compute_output(1), want_b = has_bias && task_should_compute_output(2);
         if (want_x || want_w || want_b) {
             static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::linear_act_bwd", "").typed<linear_act_bwd_symbolic>();
             // unpacked before the guard, as above
-            const Tensor kept = slope.unpack();
-            const OptTensor x_in = want_w ? OptTensor(x.unpack()) : OptTensor(), weight_in = want_x ? OptTensor(weight.unpack()) : OptTensor();
-            at::AutoDispatchBelowADInplaceOrView below;
-            auto d = op.call(grads[0], kept, x_in, weight_in, shape, out, bias_dtype, want_x, want_w, want_b);
+            const Tensor kept = slope.unpack(), x_in = want_w ? x.unpack() : Tensor(), weight_in = want_x ? weight.unpack() : Tensor();
+            const BelowAutograd below(in_transform("linear_act", grads[0], kept, x_in, weight_in));
+            auto d = op.call(grads[0], kept, want_w ? OptTensor(x_in) : OptTensor(), want_x ? OptTensor(weight_in) : OptTensor(), shape, out,
+                             bias_dtype, want_x, want_w, want_b);
             if (want_x) result[0] = std::get<0>(d);
             if (want_w) result[1] = std::get<1>(d);
             if (want_b) result[2] = std::get<2>(d);
@@ -507,13 +553,29 @@ struct LinearBackward : torch::autograd::Node {
     }
 };
 
-Tensor linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int64_t function,
-                       int64_t degree, int64_t source) {
+std::tuple<Tensor, Tensor, Tensor> linear_act_bwd_autograd(const Tensor& dy, const Tensor& slope, const OptTensor& x, const OptTensor& weight,
+                                                           c10::SymIntArrayRef x_shape, c10::SymInt out, int64_t bias_dtype, bool want_x,
+                                                           bool want_weight, bool want_bias) {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::linear_act_bwd", "").typed<linear_act_bwd_symbolic>();
+    const Tensor xs = x.value_or(Tensor()), ws = weight.value_or(Tensor());
+    no_forward_gradient("linear_act_bwd", dy, slope, xs, ws);
+    std::tuple<Tensor, Tensor, Tensor> d;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        d = op.call(dy, slope, x, weight, x_shape, out, bias_dtype, want_x, want_weight, want_bias);
+    }
+    refuse_to_go_on("linear_act", {std::get<0>(d), std::get<1>(d), std::get<2>(d)}, dy, slope, xs, ws);
+    return d;
+}
+
+// what a training step runs: the result with its node, and the slope (empty where nobody asks for it)
+std::tuple<Tensor, Tensor> linear_recorded(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
+                                           int64_t function, int64_t degree, int64_t source, bool want_slope) {
     static const auto with_slope = c10::Dispatcher::singleton().findSchemaOrThrow("fpt_b200::linear_act_slope", "").typed<decltype(linear_act_slope)>();
     const Tensor b = bias.value_or(Tensor()), r = residual.value_or(Tensor());
     no_forward_gradient("linear_act", x, weight, b, r);
     std::shared_ptr<LinearBackward> node;
-    bool keep_slope = false;            // no activation: the slope is 1; only the residual wants a gradient: nobody asks for it
+    bool keep_slope = want_slope;       // no activation: the slope is 1; only the residual wants a gradient: nobody asks for it
     if (torch::autograd::compute_requires_grad(x, weight, b, r)) {
         node = std::shared_ptr<LinearBackward>(new LinearBackward(), torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(x, weight, b, r));
@@ -523,20 +585,32 @@ Tensor linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& b
         node->out = weight.dim() ? weight.sym_size(0) : c10::SymInt(0);
         node->has_bias = b.defined();
         node->bias_dtype = b.defined() ? dtype_id(b.scalar_type()) : FPT_FP32;
-        keep_slope = function != FPT_FN_NONE && (x.requires_grad() || weight.requires_grad() || (b.defined() && b.requires_grad()));
+        keep_slope |= function != FPT_FN_NONE && (x.requires_grad() || weight.requires_grad() || (b.defined() && b.requires_grad()));
     }
     Tensor out, slope;
     {
         at::AutoDispatchBelowADInplaceOrView below;
         if (keep_slope) std::tie(out, slope) = with_slope.call(x, weight, bias, residual, function, degree, source);
         else out = call_linear(x, weight, bias, residual, function, degree, source);
-        if (node && !keep_slope) slope = at::empty({0, 8}, x.options().dtype(at::kHalf));
+        if (node && !keep_slope) slope = out.new_empty({0, 8}, at::TensorOptions().dtype(at::kHalf));
     }
     if (node) {
         node->slope = SavedVariable(slope, false);
         torch::autograd::set_history(out, node);
     }
-    return out;
+    return {out, slope};
+}
+
+Tensor linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual, int64_t function,
+                       int64_t degree, int64_t source) {
+    return std::get<0>(linear_recorded(x, weight, bias, residual, function, degree, source, false));
+}
+
+std::tuple<Tensor, Tensor> linear_slope_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias, const OptTensor& residual,
+                                                 int64_t function, int64_t degree, int64_t source) {
+    auto both = linear_recorded(x, weight, bias, residual, function, degree, source, true);
+    refuse_to_go_on("linear_act", {std::get<1>(both)}, x, weight, bias.value_or(Tensor()), residual.value_or(Tensor()));
+    return both;
 }
 
 // the eager doors: off the GPU the checks run here, where no kernel would be found
@@ -577,7 +651,10 @@ TORCH_LIBRARY_IMPL(fpt_b200, CUDA, m) {
 
 TORCH_LIBRARY_IMPL(fpt_b200, Autograd, m) {
     m.impl("qk_rope", &qk_rope_autograd);
+    m.impl("qk_norm_rope_bwd", &qk_norm_rope_bwd_autograd);
     m.impl("linear_act", &linear_autograd);
+    m.impl("linear_act_slope", &linear_slope_autograd);
+    m.impl("linear_act_bwd", &linear_act_bwd_autograd);
 }
 
 void register_block_operators(pybind11::module_& m) {

@@ -8,6 +8,7 @@ cores' pair form.
 
 Differentiable for x, weight, bias and residual.  A training step keeps the slope of the activation in fp16 beside x and
 the weight (nothing where there is no activation); the gradients of x and of the weight are products of the same kernels.
+A second derivative and forward-mode differentiation are refused (RuntimeError).
 Usable under `torch.compile` (`torch.ops.fpt_b200.linear_act`) and in captured graphs (what `qk_rope` says of captured backward
 passes holds here too).
 """

@@ -14,7 +14,9 @@ is fp32 with one rounding at the end, whatever the dtype (float16, bfloat16 or f
 Forward and backward pass can be captured into CUDA graphs; drop every eager graph of the same leaves before a backward pass is
 captured, as for PyTorch's own operators (a leaf's gradient accumulation stays on the stream of the graph that made it).
 
-A second derivative is refused (RuntimeError); so is a call whose shapes, dtypes or devices do not fit.
+A second derivative through the norm is refused (RuntimeError; the rotation alone is linear and has every derivative), and so are
+forward-mode differentiation and a call whose shapes, dtypes or devices do not fit.  `torch.func.grad`, `vjp` and `jacrev` and both
+forms of activation checkpointing can be used.
 """
 from __future__ import annotations
 

@@ -153,3 +153,94 @@ def test_compiled_training_step_with_any_number_of_rows(cpu_kernels, call, make,
             got = torch.autograd.grad(compiled(*args).float().sum(), args)
             assert all(torch.equal(a, b) for a, b in zip(got, want)), rows
     torch._dynamo.reset()
+
+
+def cpu_rotation(q, k):
+    return torch.cat(torch.ops.fpt_b200.qk_rope(q, k, None, None, torch.zeros(32, dtype=torch.int32), None, [], 0, 0, False, 0.0, False), dim=2)
+
+
+CALLS = {"layer": (layer, layer_args), "heads": (cpu_heads, heads_args), "rotation": (cpu_rotation, lambda rows: heads_args(rows)[:2])}
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_function_transforms_give_the_gradients_of_autograd(cpu_kernels, name):
+    call, make = CALLS[name]
+    args = make(5)
+    every = tuple(range(len(args)))
+    cotangent = values(*call(*args).shape, seed=9, grad=False)
+    want = torch.autograd.grad(call(*args), args, cotangent)
+    plain = [t.detach() for t in args]
+    loss = lambda *a: (call(*a) * cotangent).sum()
+    assert all(torch.equal(a, b) for a, b in zip(torch.func.grad(loss, argnums=every)(*plain), want))
+    y, pull = torch.func.vjp(call, *plain)
+    assert torch.equal(y, call(*plain)) and all(torch.equal(a, b) for a, b in zip(pull(cotangent), want))
+    rows = torch.func.jacrev(lambda t: call(t, *plain[1:]).flatten()[:3])(plain[0])
+    for i in range(3):
+        one = torch.zeros_like(cotangent)
+        one.view(-1)[i] = 1
+        assert torch.equal(rows[i], torch.autograd.grad(call(*args), args[0], one)[0])
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_a_transform_in_a_transform(cpu_kernels, name):
+    """The outer transform sees the inner one's value as it sees a plain call, and no second derivative that is not there."""
+    call, make = CALLS[name]
+    plain = [t.detach() for t in make(5)]
+    loss = lambda a, b: call(a, b, *plain[2:]).float().square().sum()
+    inner = lambda a, b: torch.func.grad_and_value(loss)(a, b)
+    want = torch.func.grad(loss, argnums=1)(*plain[:2])
+    assert torch.equal(torch.func.grad(lambda b: inner(plain[0], b)[1])(plain[1]), want)
+    if name != "rotation":
+        with pytest.raises(RuntimeError, match="no second gradient"):
+            torch.func.grad(lambda b: inner(plain[0], b)[0].float().sum())(plain[1])
+        with pytest.raises(RuntimeError, match="no second gradient"):
+            torch.func.grad(lambda a: inner(a, plain[1])[0].float().sum())(plain[0])
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.hessian(loss)(*plain[:2])
+
+
+def test_the_rotation_alone_has_every_derivative(cpu_kernels):
+    """It is linear: its gradient is the rotation backwards, which has a gradient.  The second derivative of a sum of squares."""
+    q, k = heads_args(3)[:2]
+    loss = lambda q: cpu_rotation(q, k.detach()).double().square().sum()
+    second = torch.func.grad(lambda q: torch.func.grad(loss)(q).double().sum())(q.detach())
+    assert torch.equal(second, torch.full_like(q, 2))
+    first, = torch.autograd.grad(loss(q), q, create_graph=True)
+    assert torch.equal(torch.autograd.grad(first.double().sum(), q)[0], torch.full_like(q, 2))
+
+
+@pytest.mark.parametrize("activation", [GELU, -1])
+@pytest.mark.parametrize("which", range(4))
+def test_vjp_of_one_argument(activation, which):
+    """Shapes only: the plain form above knows GELU alone."""
+    args = [meta(*s) for s in LAYER]
+
+    def call(t):
+        return torch.ops.fpt_b200.linear_act(*args[:which], t, *args[which + 1:], activation, 0, 0)
+    y, pull = torch.func.vjp(call, args[which])
+    assert pull(torch.empty_like(y))[0].shape == args[which].shape
+
+
+@pytest.mark.parametrize("name", ["layer", "heads"])
+def test_create_graph_is_refused(cpu_kernels, name):
+    call, make = CALLS[name]
+    args = make(5)
+    with pytest.raises(RuntimeError, match="no second gradient"):
+        torch.autograd.grad(call(*args).float().sum(), args[:1], create_graph=True)
+
+
+def test_the_parts_of_a_training_step_are_recorded(cpu_kernels):
+    """Called by themselves: the result has the layer's gradient, the slope and the gradients refuse theirs."""
+    x, w, b, r = layer_args(4)
+    y, slope = torch.ops.fpt_b200.linear_act_slope(x, w, b, r, GELU, 0, 0)
+    dy = torch.ones_like(y)
+    assert all(torch.equal(s, t) for s, t in zip(torch.autograd.grad(y, (x, w, b, r), dy), torch.autograd.grad(layer(x, w, b, r), (x, w, b, r), dy)))
+    with pytest.raises(RuntimeError, match="no second gradient"):
+        torch.autograd.grad(slope.float().sum(), x)
+    dx, *_ = torch.ops.fpt_b200.linear_act_bwd(dy, slope.detach(), x, w, x.shape, 24, 1, True, True, True)
+    with pytest.raises(RuntimeError, match="no second gradient"):
+        torch.autograd.grad(dx.float().sum(), w)
+    q, k, qw, kw = heads_args(3)
+    dq, *_ = torch.ops.fpt_b200.qk_norm_rope_bwd(q.detach(), k.detach(), q, k, qw, kw, torch.zeros(32, dtype=torch.int32), None, [], 0, 0, 1e-6, True, True)
+    with pytest.raises(RuntimeError, match="no second gradient"):
+        torch.autograd.grad(dq.float().sum(), q)

@@ -298,3 +298,31 @@ def test_a_checkpointed_patched_feed_forward(cuda):
     y = x + checkpoint(model, x, use_reentrant=False)
     got = torch.autograd.grad(y, [x, *model.parameters()], torch.ones_like(x))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_function_transforms(cuda):
+    """torch.func gives the bits of autograd; the rotation alone, which is linear, has a second derivative too (of half the sum of
+    squares: the rotation there and back, three roundings to fp32 of values below 6: 2^-18)."""
+    w, x, inc, positions, _ = case(cuda, False)
+    names = ("up", "up_bias", "q_norm")
+
+    def loss(x, up, up_bias, q_norm):
+        hidden = linear_act(x, up, up_bias, activation="gelu")[..., :768].unflatten(-1, (6, D))
+        q, k = qk_rope.qk_norm_rope(hidden[..., :4, :], hidden[..., 4:, :], q_norm, None, inc, positions=positions, pairing="halves")
+        return q.float().square().sum() + k.float().sum()
+
+    args = [t.detach() for t in (x, *(w[n] for n in names))]
+    leaves = [t.detach().requires_grad_() for t in args]
+    want = torch.autograd.grad(loss(*leaves), leaves)
+    assert all(torch.equal(a, b) for a, b in zip(torch.func.grad(loss, argnums=(0, 1, 2, 3))(*args), want))
+    value, pull = torch.func.vjp(loss, *args)
+    assert all(torch.equal(a, b) for a, b in zip(pull(torch.ones_like(value)), want))
+    with pytest.raises(RuntimeError, match="no second gradient"):
+        torch.func.grad(lambda x: torch.func.grad(loss)(x, *args[1:]).float().sum())(args[0])
+    with pytest.raises(RuntimeError, match="forward-mode"):
+        torch.func.jvp(lambda x: loss(x, *args[1:]), (args[0],), (args[0],))
+    q, k = torch.randn(1, 9, 2, D, device=cuda, requires_grad=True), torch.randn(1, 9, 1, D, device=cuda)
+    half = lambda q: 0.5 * qk_rope.rope_axes(q, k, inc, torch.arange(9, device=cuda)[None], [D // 2])[0].square().sum()
+    first, = torch.autograd.grad(half(q), q, create_graph=True)
+    second, = torch.autograd.grad(first, q, torch.ones_like(q))
+    assert (second - 1).abs().max() <= 2.0 ** -18 and (first - q).abs().max() <= 2.0 ** -18
