@@ -41,9 +41,19 @@ int make_tensor_map_bf16_4d(CUtensorMap* map, const void* base, const uint64_t d
     cuuint64_t gstride[3] = {strides_bytes[0], strides_bytes[1], strides_bytes[2]};
     cuuint32_t box[4] = {64u, box_rows, box_depth, 1u};
     cuuint32_t estride[4] = {1u, 1u, 1u, 1u};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), gdim, gstride, box, estride,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const auto run = [&] {
+        return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), gdim, gstride, box, estride,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = run();
+    if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+        // A host thread that has made no runtime call that needs the device has no context yet, which this driver call does not
+        // make by itself: bind the thread to its own current device.
+        int device = 0;
+        if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return FPT_ERR_NO_DEVICE;
+        r = run();
+    }
     return r == CUDA_SUCCESS ? FPT_OK : FPT_ERR_BAD_SIZE;
 }
 

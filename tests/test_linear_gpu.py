@@ -401,3 +401,27 @@ def test_compiled_training_step_with_any_number_of_rows(cuda):
             got = torch.autograd.grad(compiled(*leaves), leaves, dy)
             assert all(torch.equal(a, b) for a, b in zip(got, want)), rows
     torch._dynamo.reset()
+
+
+def test_a_thread_that_has_made_no_call_yet(cuda, fpt):
+    """The first call of a new host thread is the layer's, through the C ABI and through the operator (its output comes from the
+    allocator's cache): the thread has no context of its own before it."""
+    import threading
+    lib, (x, w, b, _, _) = fpt.load(), inputs(300, 64, 24, torch.bfloat16, cuda)
+    want, out, got = linear_act(x, w, b, activation="gelu"), torch.empty(300, 24, dtype=torch.bfloat16, device=cuda), []
+    spare = torch.empty_like(out)
+    del spare
+    stream = torch.cuda.current_stream().cuda_stream
+    torch.cuda.synchronize()
+    calls = [lambda: lib.fpt_linear(out.data_ptr(), None, x.data_ptr(), w.data_ptr(), b.data_ptr(), None, 300, 64, 24, 64, 64, 24, 0, 0, 1, 1, 4,
+                                    0, 0, None, stream),
+             lambda: linear_act(x, w, b, activation="gelu")]
+    for call in calls:
+        thread = threading.Thread(target=lambda: got.append(call()))
+        thread.start()
+        thread.join()
+    torch.cuda.synchronize()
+    assert got[0] == 0 and len(got) == 2
+    assert torch.equal(out, want) and torch.equal(got[1], want)
+
+
