@@ -946,11 +946,13 @@ struct Product {
     bool a_mn, b_mn;                   // operand stored [k, rows] instead of [rows, k]
 };
 
-// A launch that may begin while the kernel before it in the stream drains; `cluster` 0: the kernel's own attribute, or none.
+// A launch that may begin while the kernel before it in the stream drains; `cluster` 0: the kernel's own attribute, or none.  The
+// kernel's limit of shared memory belongs to all threads of the process: it is set to `smem_most`, which is the same in every
+// call of a kernel, so that no thread lowers it between another's setting and launch.
 template <class... P, class... A>
-cudaError_t launch_early(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, unsigned cluster, cudaStream_t stream, const A&... args) {
-    if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+cudaError_t launch_early(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, size_t smem_most, unsigned cluster, cudaStream_t stream, const A&... args) {
+    if (smem_most > 48 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem_most));
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t config{};
@@ -1047,8 +1049,8 @@ int launch_pair(const Product& q, LinearParams& p, const DeviceInfo& dev, PairFo
     const int64_t pairs = p.split > 1 ? tiles * p.split : std::min<int64_t>(tiles, dev.sm_count / 2);
     if (pairs > 0x3fffffff) return FPT_ERR_BAD_SIZE;
     if (p.split > 1)
-        return cuda_status(launch_early(linear_shared_pair_kernel<DT, ACT, SLOPE, A_MN, B_MN>, unsigned(2 * pairs), kPairThreads, smem, unsigned(2 * p.split), stream, map_a, map_b, p));
-    return cuda_status(launch_early(linear_pair_kernel<DT, ACT, SLOPE, A_MN, B_MN>, unsigned(2 * pairs), kPairThreads, smem, 0u, stream, map_a, map_b, p));
+        return cuda_status(launch_early(linear_shared_pair_kernel<DT, ACT, SLOPE, A_MN, B_MN>, unsigned(2 * pairs), kPairThreads, smem, smem, unsigned(2 * p.split), stream, map_a, map_b, p));
+    return cuda_status(launch_early(linear_pair_kernel<DT, ACT, SLOPE, A_MN, B_MN>, unsigned(2 * pairs), kPairThreads, smem, smem, 0u, stream, map_a, map_b, p));
 }
 
 // Whether a block of the few-row form takes all of an SM's shared memory: where every block can have an SM to itself (clusters do
@@ -1069,10 +1071,13 @@ int launch_split(const Product& q, LinearParams& p, const DeviceInfo& dev, int s
     const int64_t blocks = int64_t(p.m_tiles) * p.n_tiles * split;
     if (blocks > 0x7fffffff) return FPT_ERR_BAD_SIZE;
     const uint32_t stage = kTileBytes + TOKENS * 128;
-    const uint32_t budget = alone_on_sm(blocks, split, dev.sm_count) ? 216u * 1024u : 108u * 1024u;
+    constexpr uint32_t kRingMost = 216 * 1024, kRingHalf = 108 * 1024;     // of a block alone on its SM, of one of two
+    constexpr size_t kSmemMost = 1024 + kSplitRingOffset + kRingMost;
+    static_assert(TOKENS * 512 <= kRingHalf && kSmemMost <= 227 * 1024, "shared memory budget");
+    const uint32_t budget = alone_on_sm(blocks, split, dev.sm_count) ? kRingMost : kRingHalf;
     p.ring = int(std::min<uint32_t>(kMaxRing, budget / stage));
     const size_t smem = 1024 + kSplitRingOffset + std::max<size_t>(size_t(p.ring) * stage, size_t(TOKENS) * 512);
-    return cuda_status(launch_early(linear_split_kernel<DT, ACT, SLOPE, TOKENS, W_MN>, unsigned(blocks), kSplitThreads, smem,
+    return cuda_status(launch_early(linear_split_kernel<DT, ACT, SLOPE, TOKENS, W_MN>, unsigned(blocks), kSplitThreads, smem, kSmemMost,
                                       split > 1 ? unsigned(split) : 0u, stream, map_w, map_x, p));
 }
 
@@ -1314,10 +1319,10 @@ extern "C" int fpt_linear_grad_act(void* dz, void* dbias, const void* dy, const 
         p.vec_dy = aligned16(dy, dy_ld);
         chunks = int((rows + p.chunk_rows - 1) / p.chunk_rows);
         const dim3 grid(unsigned((out_features + kActColumns - 1) / kActColumns), unsigned(chunks));
-        if (int rc = cuda_status(launch_early(dtype == FPT_BF16 ? linear_grad_act_kernel<kBf16> : linear_grad_act_kernel<kFp16>, grid, kActThreads, 0, 0u, stream, p))) return rc;
+        if (int rc = cuda_status(launch_early(dtype == FPT_BF16 ? linear_grad_act_kernel<kBf16> : linear_grad_act_kernel<kFp16>, grid, kActThreads, 0, 0, 0u, stream, p))) return rc;
     }
     if (dbias) {
-        return cuda_status(launch_early(linear_bias_grad_kernel, unsigned((out_features + 31) / 32), 256u, 0, 0u, stream,
+        return cuda_status(launch_early(linear_bias_grad_kernel, unsigned((out_features + 31) / 32), 256u, 0, 0, 0u, stream,
                                         static_cast<const float*>(workspace), dbias, chunks, int(out_features), bias_dtype));
     }
     return FPT_OK;

@@ -425,3 +425,32 @@ def test_a_thread_that_has_made_no_call_yet(cuda, fpt):
     assert torch.equal(out, want) and torch.equal(got[1], want)
 
 
+def test_threads_with_rings_of_two_sizes(cuda, fpt):
+    """One kernel with a ring of 216 KB (a block alone on its SM) and of 108 KB, from threads that call at once (ctypes lets go of
+    the interpreter's lock).  No launch fails on a limit that another thread set."""
+    import threading
+    lib, args = fpt.load(), [inputs(1, n, n, torch.bfloat16, cuda, residual=False)[:3] for n in (4096, 1024)]
+    want = [linear_act(*a, activation="gelu") for a in args]
+    made, failures, start = [], [], threading.Barrier(4)
+    torch.cuda.synchronize()
+
+    def run(i):
+        x, w, b = args[i % 2]
+        n, out, stream = x.shape[1], torch.zeros_like(x), torch.cuda.Stream(cuda)
+        call = (out.data_ptr(), None, x.data_ptr(), w.data_ptr(), b.data_ptr(), None, 1, n, n, n, n, n, 0, 0, 1, 1, 4, 0, 0, None, stream.cuda_stream)
+        made.append((i, out, stream))
+        start.wait()
+        for _ in range(5000):
+            status = lib.fpt_linear(*call)
+            if status:
+                failures.append(status)
+                return
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    torch.cuda.synchronize()
+    assert not failures
+    assert len(made) == 4 and all(torch.equal(out, want[i % 2]) for i, out, _ in made)
