@@ -1,7 +1,7 @@
 // A linear layer with everything that follows it in the epilogue, for sm_100a: y = act(x W^T + b) + r, and the products and
 // the element-wise pass of its gradient.
 //
-//   forward          y [rows, out]  = act(x [rows, dim] W[out, dim]^T + b) + r,   optionally act'(x W^T + b) in fp16
+//   forward          y [rows, out]  = act(x [rows, dim] W[out, dim]^T + b) + r,   optionally 2^15 act'(x W^T + b) in fp16
 //   dz = dy act'     element-wise, with the column sums that are the gradient of b
 //   dx [rows, dim] = dz W           the contraction runs over W's rows: W is an MN-major operand
 //   dW [out, dim]  = dz^T x         both operands MN-major
@@ -25,9 +25,10 @@
 //   linear_grad_act_kernel  6 bytes a value: 4096 x 4096 bf16 18.1 us = 5.6 TB/s, with the column sums 20.5.
 //
 // Rounding: the epilogue works on the fp32 accumulators and rounds once.  The slope act' is kept in fp16 also beside bf16
-// data: it lies in about [-0.13, 1.13], where fp16 has eight times the resolution of bf16 at the same size, so the backward
-// pass adds no error of bf16's size by it (z itself in bf16 would).  dz is rounded to the data type before the two
-// products, which take 16-bit operands; its column sums are taken before that rounding.
+// data, times 2^15: it lies in about [-0.13, 1.14], so 2^15 keeps it below fp16's largest value, and down to 2^-29 it has eight
+// times the resolution of bf16 (half a step is 2^-11 of it; below that 2^-40 whatever its size): the backward pass adds no
+// error of bf16's size by it (z itself in bf16 would).  dz is rounded to the data type before the two products, which take
+// 16-bit operands; its column sums are taken before that rounding.
 // The polynomial forms (degree 3 .. 6) run the packed 16-bit programs of fpt_unary on z rounded to the data type: what a
 // separate product followed by fpt_unary gives, bit for bit.
 // Every mbarrier wait is bounded; a wait that runs out writes a word the host can read without a copy and unwinds.
@@ -54,6 +55,8 @@ constexpr int kBandTiles = 16;                      // 256-row tiles per band: 4
 enum : uint32_t { kWaitEmpty = 0x51, kWaitFull, kWaitAccEmpty, kWaitAccFull };
 enum Act : int { kNone, kSigmoid, kTanh, kSwishAct, kGelu, kProgram };   // compile-time: one straight piece of code each
 
+constexpr float kSlopeScale = 32768.0f;             // of act' as it is stored
+
 struct Programs {                      // of kProgram
     int fwd_shape, fwd_degree, bwd_shape, bwd_degree;
     ProgramWords fwd, bwd;
@@ -63,7 +66,7 @@ struct LinearParams {
     void* out;                      // [m, n] rows of out_ld
     const void* residual;           // [m, n] or null
     const void* bias;               // [n] or null
-    uint16_t* slope;                // [m, n] fp16 or null
+    uint16_t* slope;                // [m, n] fp16, kSlopeScale act', or null
     int64_t out_ld, res_ld, slope_ld;
     int m, n, k_blocks;             // k_blocks: of 64 (split form), of 64 chunks (pair form)
     int m_tiles, n_tiles;
@@ -144,18 +147,27 @@ __device__ __forceinline__ float normal_tail(float a, float e) {
     q = fmaf(t, q, 0.105599835f);
     return q * t * e;
 }
-// tanh: the quotient of exponentials, and where that cancels (|z| < 0.3) its series to z^9 (next term < 2^-24 of z)
-__device__ __forceinline__ float tanh_of(float z) {
-    const float far = fmaf(-2.0f, mufu_rcp(1.0f + mufu_ex2(2.8853900817779268f * z)), 1.0f);
+// tanh: the quotient of exponentials, and where that cancels (|z| < 0.3) its series to z^9 (next term < 2^-24 of z).  Its slope
+// (times kSlopeScale) is 4 r (1 - r) with r = 1 / (1 + e^2z), and 1 - r is e^2z r where r is near 1: 1 - tanh^2 would cancel.
+template <bool SLOPE>
+__device__ __forceinline__ float tanh_of(float z, float& slope) {
+    const float e = mufu_ex2(2.8853900817779268f * z), r = mufu_rcp(1.0f + e);
+    if constexpr (SLOPE) slope = 4.0f * kSlopeScale * r * (z < 0.0f ? e * r : 1.0f - r);
+    const float far = fmaf(-2.0f, r, 1.0f);
     const float q = z * z;
     float s = fmaf(q, 2.1869488536e-2f, -5.3968253968e-2f);
     s = fmaf(q, s, 1.3333333333e-1f);
     s = fmaf(q, s, -3.3333333333e-1f);
     return fabsf(z) < 0.3f ? fmaf(z * q, s, z) : far;
 }
-__device__ __forceinline__ float logistic(float z) { return mufu_rcp(1.0f + mufu_ex2(-1.4426950408889634f * z)); }
+// q = logistic(z), and 1 - q without cancelling
+__device__ __forceinline__ float logistic(float z, float& rest) {
+    const float e = mufu_ex2(-1.4426950408889634f * z), q = mufu_rcp(1.0f + e);
+    rest = z > 0.0f ? e * q : 1.0f - q;
+    return q;
+}
 
-// z -> act(z), d -> act'(z) where wanted
+// z -> act(z), d -> act'(z) kSlopeScale where wanted
 template <int DT, int ACT, bool SLOPE, int N>
 __device__ __forceinline__ void activate(const Programs& a, float (&z)[N], float (&d)[N]) {
     if constexpr (ACT == kProgram) {
@@ -167,8 +179,8 @@ __device__ __forceinline__ void activate(const Programs& a, float (&z)[N], float
             z[i + 1] = Sfu<DT>::hi(y);
             if constexpr (SLOPE) {
                 const uint32_t s = run_program<DT>(x, a.bwd, a.bwd_shape, a.bwd_degree);
-                d[i] = Sfu<DT>::lo(s);
-                d[i + 1] = Sfu<DT>::hi(s);
+                d[i] = Sfu<DT>::lo(s) * kSlopeScale;
+                d[i + 1] = Sfu<DT>::hi(s) * kSlopeScale;
             }
         }
     } else if constexpr (ACT != kNone) {
@@ -179,14 +191,14 @@ __device__ __forceinline__ void activate(const Programs& a, float (&z)[N], float
                 const float e = mufu_ex2(-0.72134752044448170368f * x * x), tail = normal_tail(fabsf(x), e);
                 const float phi = x < 0.0f ? tail : 1.0f - tail;
                 z[i] = x * phi;
-                if constexpr (SLOPE) d[i] = fmaf(x * 0.3989422804014327f, e, phi);
+                if constexpr (SLOPE) d[i] = fmaf(x * 0.3989422804014327f, e, phi) * kSlopeScale;
             } else if constexpr (ACT == kTanh) {
-                z[i] = tanh_of(x);
-                if constexpr (SLOPE) d[i] = fmaf(-z[i], z[i], 1.0f);
+                z[i] = tanh_of<SLOPE>(x, d[i]);
             } else {
-                const float q = logistic(x);
+                float rest;
+                const float q = logistic(x, rest);
                 z[i] = ACT == kSwishAct ? x * q : q;
-                if constexpr (SLOPE) d[i] = ACT == kSwishAct ? q * fmaf(x, 1.0f - q, 1.0f) : q * (1.0f - q);
+                if constexpr (SLOPE) d[i] = q * kSlopeScale * (ACT == kSwishAct ? fmaf(x, rest, 1.0f) : rest);
             }
         }
     }
@@ -827,7 +839,7 @@ constexpr int kActBlocks = 5;           // resident on an SM, at 48 registers (a
 
 struct GradActParams {
     const uint16_t* dy;
-    const uint16_t* slope;              // fp16, or null for 1
+    const uint16_t* slope;              // fp16, kSlopeScale act', or null for 1
     uint16_t* dz;                       // or null
     float* partial;                     // [chunks, out] column sums, or null
     int64_t dy_ld, slope_ld, dz_ld;
@@ -869,8 +881,8 @@ __global__ void __launch_bounds__(kActThreads) linear_grad_act_kernel(const Grad
                 s[0] = w.x, s[1] = w.y, s[2] = w.z, s[3] = w.w;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    v[2 * i] = 2 * i < live ? v[2 * i] * Sfu<kFp16>::lo(s[i]) : 0.0f;
-                    v[2 * i + 1] = 2 * i + 1 < live ? v[2 * i + 1] * Sfu<kFp16>::hi(s[i]) : 0.0f;
+                    v[2 * i] = 2 * i < live ? v[2 * i] * (Sfu<kFp16>::lo(s[i]) * (1.0f / kSlopeScale)) : 0.0f;
+                    v[2 * i + 1] = 2 * i + 1 < live ? v[2 * i + 1] * (Sfu<kFp16>::hi(s[i]) * (1.0f / kSlopeScale)) : 0.0f;
                 }
             }
             if (p.dz) {

@@ -4,7 +4,7 @@
 //   fpt_b200::qk_rope            norm of every head and rotation, or the rotation alone (fpt_qk_rope)
 //   fpt_b200::qk_norm_rope_bwd   gradient of the form with the norm
 //   fpt_b200::linear_act         act(x W^T + b) + r (fpt_linear)
-//   fpt_b200::linear_act_slope   the same with act' beside it, what a training step keeps
+//   fpt_b200::linear_act_slope   the same with 2^15 act' in fp16 beside it, what a training step keeps
 //   fpt_b200::linear_act_bwd     its gradient (fpt_linear_grad_act, _grad_input, _grad_weight)
 //
 // The Python module enters through plain functions that check the arguments that are not tensors and call the dispatcher

@@ -6,8 +6,9 @@ The activation and the residual are applied to the fp32 sums in registers and ro
 the result is stored.  Any number of rows: one token streams the weight at the memory's rate, many rows run on the tensor
 cores' pair form.
 
-Differentiable for x, weight, bias and residual.  A training step keeps the slope of the activation in fp16 beside x and
-the weight (nothing where there is no activation); the gradients of x and of the weight are products of the same kernels.
+Differentiable for x, weight, bias and residual.  A training step keeps the slope of the activation in fp16 (times 2^15, so
+that small slopes keep their precision) beside x and the weight (nothing where there is no activation); the gradients of x and
+of the weight are products of the same kernels.
 A second derivative and forward-mode differentiation are refused (RuntimeError).
 Usable under `torch.compile` (`torch.ops.fpt_b200.linear_act`) and in captured graphs (what `qk_rope` says of captured backward
 passes holds here too).

@@ -405,8 +405,9 @@ int fpt_qk_norm_rope_bwd(void* dq, void* dk, void* dq_weight, void* dk_weight, c
  *      function: FPT_FN_NONE, FPT_FN_SIGMOID, FPT_FN_TANH, FPT_FN_SWISH or FPT_FN_GELU.  degree 0: the function itself in
  *      fp32 on the fp32 sums, one rounding at the end.  degree 3..6: the packed polynomial program of fpt_unary on the sums
  *      rounded to dtype (with a residual: its value plus the residual, rounded again).
- *      slope (fp16 [rows, out_features], whatever dtype) or null: act'(x W^T + b) for fpt_linear_grad_act; with a degree
- *      the derivative program of the same degree; null where there is no activation.
+ *      slope (fp16 [rows, out_features], whatever dtype) or null: 2^15 act'(x W^T + b) for fpt_linear_grad_act (fp16 is
+ *      subnormal, coarser than bf16, below 2^-14; |act'| is at most 1.14); with a degree the derivative program of the same
+ *      degree; null where there is no activation.
  *      status: one word the device can write and the host can read (mapped host memory serves; null: not reported): a
  *      bounded device-side wait that runs out stores 0x80000000 | where there, and the outputs of that call are invalid.
  *      It is not read when a call starts. */
@@ -414,7 +415,7 @@ int fpt_linear(void* out, void* slope, const void* x, const void* weight, const 
                int64_t rows, int64_t dim, int64_t out_features, int64_t x_ld, int64_t w_ld, int64_t out_ld,
                int64_t residual_ld, int64_t slope_ld, int dtype, int bias_dtype, int function, int degree, int source,
                void* status, fpt_stream_t stream);
-/* Its gradient in three parts.  dz = dy * slope (slope null: dz = dy) rounded to dtype, dbias = its column sums before that
+/* Its gradient in three parts.  dz = dy * slope / 2^15 (slope null: dz = dy) rounded to dtype, dbias = its column sums before that
  *      rounding, in a fixed order; dz or dbias null where not wanted.  dz and slope rows are 16-byte aligned and padded to
  *      a multiple of 8 columns (the padding of dz is written with zeros); workspace (4-byte aligned) for dbias. */
 int64_t fpt_linear_grad_act_workspace_bytes(int64_t rows, int64_t out_features);

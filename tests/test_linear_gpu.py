@@ -454,3 +454,24 @@ def test_threads_with_rings_of_two_sizes(cuda, fpt):
     torch.cuda.synchronize()
     assert not failures
     assert len(made) == 4 and all(torch.equal(out, want[i % 2]) for i, out, _ in made)
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("activation, low, high", [("sigmoid", -26, 26), ("tanh", -13, 13), ("silu", -26, -3), ("gelu", -7, -3)])
+def test_small_slopes_keep_their_precision(cuda, activation, low, high, dtype, rows):
+    """Relative to the gradient, where the slope is small.  With the identity for a weight z = x and dx = dz, so dx is dy times the
+    slope with its roundings: h for the result, h of fp16 for the slope as it is kept (steps of 2^-10 from 1 on: 2^-11 of the value;
+    below 2^-29, where 2^15 times the slope is subnormal, steps of 2^-24 2^-15: 2^-40), and what the exponential carries.  That is the rounding of its argument, at most 4 |z| u in sigmoid, SiLU and tanh and
+    2 z^2 u in GELU, and 16 u for ex2, rcp and the products."""
+    w = torch.eye(64, device=cuda).to(DTYPES[dtype])
+    x = torch.linspace(low, high, rows * 64, device=cuda).reshape(rows, 64).to(DTYPES[dtype])
+    dy = torch.randn(rows, 64, device=cuda).to(DTYPES[dtype])
+    leaf = x.detach().requires_grad_()
+    dx, = torch.autograd.grad(linear_act(leaf, w, activation=activation), leaf, dy)
+    z, d = x.double(), dy.double()
+    want = d * (torch.sigmoid(z) * torch.sigmoid(-z) if activation == "sigmoid" else act_and_slope(z, activation)[1])   # 1 - p would cancel
+    rel, least = half(DTYPES[dtype])
+    exponential = (2 * z * z if activation == "gelu" else 4 * z.abs()) + 16
+    slack = (2.0 ** -11 + exponential * U) * want.abs() + 2.0 ** -40 * d.abs()
+    assert ((dx.double() - want).abs() <= rel * (want.abs() + slack) + slack + least).all()
