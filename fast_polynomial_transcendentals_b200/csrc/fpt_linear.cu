@@ -86,7 +86,8 @@ struct LinearParams {
 // ---- waits --------------------------------------------------------------------------------------------------------
 
 // Launched while the kernel before it drains (launch_early below): barriers and tensor memory are set up by then, and nothing of
-// global memory is touched before this.
+// global memory is touched before this.  What that kernel writes changes during this one's life, so nothing is read as constant
+// (no __ldg, no __restrict__: such a load may be moved ahead of the wait).
 __device__ __forceinline__ void wait_for_inputs() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -909,7 +910,7 @@ __global__ void __launch_bounds__(kActThreads) linear_grad_act_kernel(const Grad
 }
 
 // the chunks' sums, always in the same order
-__global__ void __launch_bounds__(256) linear_bias_grad_kernel(const float* __restrict__ partial, void* out, int chunks, int n, int dtype) {
+__global__ void __launch_bounds__(256) linear_bias_grad_kernel(const float* partial, void* out, int chunks, int n, int dtype) {
     __shared__ float part[8][33];
     wait_for_inputs();
     const int column = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;

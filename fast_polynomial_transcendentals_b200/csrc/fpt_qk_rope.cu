@@ -44,7 +44,8 @@ template <class T, bool NORM>
 constexpr int kFwdBlocks = sizeof(T) == 4 ? 2 : NORM ? 3 : 4;
 constexpr int kBwdBlocks = 2;
 
-// Launched while the kernel before it drains; nothing of global memory is touched before this.
+// Launched while the kernel before it drains; nothing of global memory is touched before this.  What that kernel writes changes
+// during this one's life, so nothing is read as constant (no __ldg, no __restrict__: such a load may be moved ahead of the wait).
 __device__ __forceinline__ void wait_for_inputs() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -330,7 +331,7 @@ __device__ __forceinline__ uint32_t load_position(const QkRopeArgs& a, uint32_t 
     const uint32_t b = a.seq.div(token), s = token - b * a.seq.d;
     if (!a.positions) return s;
     const int64_t from = int64_t(a.axis[pair]) * a.pos_axis + int64_t(b) * a.pos_b + int64_t(s) * a.pos_s;
-    return __ldg(static_cast<const uint32_t*>(a.positions) + from * a.pos_words);        // low word
+    return static_cast<const uint32_t*>(a.positions)[from * a.pos_words];        // low word
 }
 // where the sine and cosine of a pair lie among those of its token
 template <int C, bool HALVES>
@@ -354,7 +355,7 @@ __device__ __forceinline__ void fill_trig(Shared& sm, const QkRopeArgs& a, uint3
         for (int e = 0; e < 2; ++e) {              // both loads before either sine
             const uint32_t i = min(first + e * kThreads, n - 1), t = a.pairs.div(i), pair = i - t * a.pairs.d;
             at[e] = t * a.pairs.d + trig_place<C, HALVES>(a, pair);
-            phase[e] = load_position(a, token0 + t, pair) * __ldg(a.increments + pair);
+            phase[e] = load_position(a, token0 + t, pair) * a.increments[pair];
         }
         put_trig(sm, a, at[0], phase[0]);
         if (first + kThreads < n) put_trig(sm, a, at[1], phase[1]);
@@ -711,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_norm_rope_bwd_kernel(
 }
 
 // dw[column] = sum of the blocks' partial gradients, always in the same order
-__global__ void __launch_bounds__(256) weight_grad_kernel(const float* __restrict__ q_partial, const float* __restrict__ k_partial,
+__global__ void __launch_bounds__(256) weight_grad_kernel(const float* q_partial, const float* k_partial,
                                                           void* q_out, void* k_out, int q_blocks, int k_blocks, int dim, int dtype) {
     __shared__ float part[256];
     wait_for_inputs();

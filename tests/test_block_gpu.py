@@ -326,3 +326,39 @@ def test_function_transforms(cuda):
     first, = torch.autograd.grad(half(q), q, create_graph=True)
     second, = torch.autograd.grad(first, q, torch.ones_like(q))
     assert (second - 1).abs().max() <= 2.0 ** -18 and (first - q).abs().max() <= 2.0 ** -18
+
+
+def test_results_read_on_a_second_stream(cuda):
+    """Launches that begin while the kernel before them drains, back to back, with inputs that the kernel before has just written
+    (positions too) and results that another stream copies behind an event: the bits of calls with a wait after each."""
+    w, x0, inc, _, _ = case(cuda, False)
+
+    def run(settle, read):
+        x, pos, out = x0.clone(), torch.zeros(B, S, dtype=torch.int32, device=cuda), []
+        for _ in range(40):
+            pos.add_(997)
+            settle()
+            q, k, v = split_heads(linear_act(x, w["qkv"], w["qkv_bias"]))
+            settle()
+            q, k = qk_rope.qk_norm_rope(q, k, w["q_norm"], w["k_norm"], inc, positions=pos, pairing="halves")
+            settle()
+            out += read(q, k)
+            x = linear_act(q.flatten(2), w["out"], None, x0)
+            settle()
+            out += read(x)
+        torch.cuda.synchronize()
+        return out
+
+    side = torch.cuda.Stream(cuda)
+
+    def aside(*tensors):
+        side.wait_event(torch.cuda.current_stream().record_event())
+        with torch.cuda.stream(side):
+            for t in tensors:
+                t.record_stream(side)
+            return [t.clone() for t in tensors]
+
+    want = run(torch.cuda.synchronize, lambda *tensors: [t.clone() for t in tensors])
+    got = run(lambda: None, aside)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    check_linear_status()
