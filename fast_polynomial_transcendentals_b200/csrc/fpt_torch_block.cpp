@@ -87,7 +87,7 @@ struct BelowAutograd {
 // a tangent would be lost below the autograd keys
 template <class... T>
 void no_forward_gradient(const char* name, const T&... inputs) {
-    TORCH_CHECK(!(torch::autograd::isFwGradDefined(inputs) || ...), name, " has no forward-mode derivative");
+    TORCH_CHECK(!((inputs.defined() && inputs._fw_grad(/*level=*/0).defined()) || ...), name, " has no forward-mode derivative");
 }
 
 // ---- fpt_qk_rope --------------------------------------------------------------------------------------------------
