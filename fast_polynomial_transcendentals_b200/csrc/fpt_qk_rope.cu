@@ -26,17 +26,16 @@
 #include <type_traits>
 
 #include "fpt_common.h"
+#include "fpt_qk_rope_plan.h"
 
 namespace fpt {
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 128;
-constexpr int kMaxTileTokens = 32;
 constexpr int kMaxTrig = 2048;          // tokens x pairs of a tile
 constexpr int kMaxAxes = 4;
 constexpr int kStages = 3;              // items of a thread in its ring
-constexpr int kBwdTrig = 512;           // tokens x pairs of a tile of the backward pass (two entries a thread, two tiles)
 // Blocks an SM holds, by registers (16-bit data; 2 in fp32).  Measured: the forward pass with the norm 29.5 us at 3 and 33.3 at 4
 // (which spills), the rotation alone 51.8 at 3 and 50.8 at 4, forward and backward pass together 121 with the backward
 // pass at 3 (spills) and 87 at 2 (before the shares of share_blocks).
@@ -76,7 +75,7 @@ struct Side {                          // queries or keys
     float* partial;                    // backward: [blocks, dim] partial weight gradients, or null
     Rows xs, gs;
     uint32_t heads;
-    uint32_t blocks, tiles, tile_tokens;   // backward: blocks on this side, its tiles
+    BwdShare share;                    // backward: its tiles and blocks
 };
 struct QkRopeArgs {
     Side side[2];                      // 0 queries, 1 keys
@@ -565,9 +564,9 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_norm_rope_bwd_kernel(
     extern __shared__ __align__(16) char ring_raw[];
     __shared__ Shared sm;
     const Ring<T, C, kStages> ring_x(ring_raw), ring_g(ring_raw + Ring<T, C, kStages>::kBytes);
-    const int keys = blockIdx.x >= a.side[0].blocks;
+    const int keys = blockIdx.x >= a.side[0].share.blocks;
     const Side& side = a.side[keys];
-    const uint32_t block = keys ? blockIdx.x - a.side[0].blocks : blockIdx.x;
+    const uint32_t block = keys ? blockIdx.x - a.side[0].share.blocks : blockIdx.x;
     const int lane_unit = threadIdx.x & (G - 1);
     const bool live = lane_unit < a.units;
     const int unit = live ? lane_unit : 0;
@@ -575,22 +574,22 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_norm_rope_bwd_kernel(
     const Place at = place<C>(unit, a.rotary_units);
     const uint32_t lo = uint32_t(at.lo) * sizeof(T), hi = uint32_t(at.hi) * sizeof(T), out_bytes = uint32_t(a.dim) * sizeof(T);
     const float inv_dim = 1.0f / float(a.dim);
-    const uint32_t heads = side.heads, step = kGroups / side.tile_tokens, group = threadIdx.x / G;
+    const uint32_t heads = side.heads, step = kGroups / side.share.tile_tokens, group = threadIdx.x / G;
     const uint32_t my_slot = group / step, head = group % step, rounds = (heads + step - 1) / step;
-    const bool one = side.tile_tokens == 1;
+    const bool one = side.share.tile_tokens == 1;
     wait_for_inputs();
     // loads run ahead over the tiles: where they are
     uint32_t ahead_tile = block, ahead_round = 0, ahead_stage = 0, row = 0, row_g = 0;
     const char *x = nullptr, *grad = nullptr;
     const auto aim = [&] {
-        const uint32_t token0 = ahead_tile * side.tile_tokens, slot = min(my_slot, a.tokens - token0 - 1);
+        const uint32_t token0 = ahead_tile * side.share.tile_tokens, slot = min(my_slot, a.tokens - token0 - 1);
         x = static_cast<const char*>(side.x) + tile_base(side.xs, a, token0, one);
         grad = static_cast<const char*>(side.grad) + tile_base(side.gs, a, token0, one);
         row = tile_row(side.xs, a, token0, slot, one);
         row_g = tile_row(side.gs, a, token0, slot, one);
     };
     const auto fetch = [&] {
-        if (ahead_tile < side.tiles) {
+        if (ahead_tile < side.share.tiles) {
             const uint32_t h = min(head + ahead_round * step, heads - 1);
             const uint32_t from = row + h * side.xs.h, from_g = row_g + h * side.gs.h;
             ring_x.fetch(ahead_stage, x, from + lo, from + hi);
@@ -598,8 +597,8 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_norm_rope_bwd_kernel(
             ahead_stage = ahead_stage + 1 == kStages ? 0 : ahead_stage + 1;
             if (++ahead_round == rounds) {
                 ahead_round = 0;
-                ahead_tile += side.blocks;
-                if (ahead_tile < side.tiles) aim();
+                ahead_tile += side.share.blocks;
+                if (ahead_tile < side.share.tiles) aim();
             }
         }
         copy_commit();
@@ -616,21 +615,21 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_norm_rope_bwd_kernel(
         trig_slot[e] = a.pairs.div(i);
         trig_pair[e] = i - trig_slot[e] * a.pairs.d;
         trig_at[e] = trig_slot[e] * a.pairs.d + trig_place<C, HALVES>(a, trig_pair[e]);
-        if (trig_slot[e] >= side.tile_tokens) trig_slot[e] = 0x40000000u;              // no entry
-        increment[e] = trig_slot[e] < side.tile_tokens ? a.increments[trig_pair[e]] : 0u;
+        if (trig_slot[e] >= side.share.tile_tokens) trig_slot[e] = 0x40000000u;              // no entry
+        increment[e] = trig_slot[e] < side.share.tile_tokens ? a.increments[trig_pair[e]] : 0u;
         position[e] = 0;
     }
     const auto load_positions = [&](uint32_t tile) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const uint32_t token = tile * side.tile_tokens + trig_slot[e];
-            if (tile < side.tiles && token < a.tokens) position[e] = load_position(a, token, trig_pair[e]);
+            const uint32_t token = tile * side.share.tile_tokens + trig_slot[e];
+            if (tile < side.share.tiles && token < a.tokens) position[e] = load_position(a, token, trig_pair[e]);
         }
     };
     const auto put = [&](uint32_t half) {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-            if (trig_slot[e] < side.tile_tokens) put_trig(sm, a, half * kBwdTrig + trig_at[e], position[e] * increment[e]);
+            if (trig_slot[e] < side.share.tile_tokens) put_trig(sm, a, half * kBwdTrig + trig_at[e], position[e] * increment[e]);
     };
     load_positions(block);
     keep_weight<C>(sm.weight[0], a, fetch_weight<C, HALVES>(side, a));
@@ -641,11 +640,11 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_norm_rope_bwd_kernel(
     for (int j = 0; j < C / 2; ++j) dw.a[j] = dw.b[j] = 0;
     uint32_t half = 0, stage = 0;
 #pragma unroll 1
-    for (uint32_t tile = block; tile < side.tiles; tile += side.blocks, half ^= 1) {
-        const uint32_t token0 = tile * side.tile_tokens, count = min(side.tile_tokens, a.tokens - token0);
+    for (uint32_t tile = block; tile < side.share.tiles; tile += side.share.blocks, half ^= 1) {
+        const uint32_t token0 = tile * side.share.tile_tokens, count = min(side.share.tile_tokens, a.tokens - token0);
         const uint32_t slot = min(my_slot, count - 1), end = my_slot < count ? heads : 0u;
         char* out = static_cast<char*>(side.out) + int64_t(token0) * heads * out_bytes;
-        load_positions(tile + side.blocks);
+        load_positions(tile + side.share.blocks);
         const Angles<C> angles = lane_angles<C>(sm, a, half * kBwdTrig + slot * a.pairs.d, unit);
 #pragma unroll 1
         for (uint32_t n = 0; n < rounds; ++n) {
@@ -683,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) qk_norm_rope_bwd_kernel(
             store_run(out, to + lo, y.lo);
             store_run(out, to + hi, y.hi);
         }
-        if (tile + side.blocks < side.tiles) put(half ^ 1);
+        if (tile + side.share.blocks < side.share.tiles) put(half ^ 1);
         __syncthreads();               // the next tile's angles are there, this one's have been read
     }
     if (side.partial) {                // sum over the groups of the block, in the order of the groups, where the ring was
@@ -762,14 +761,6 @@ int group_lanes(int units) {
     int g = 4;
     while (g < units) g *= 2;
     return g;
-}
-
-// Tokens of a tile, a power of two: every group gets at least `rounds` heads of its token.  Measured for the forward pass (the
-// shapes above, us at 2, 4, 8 heads): with the norm 37.3, 29.0, 29.6; rotation alone 55.9, 50.0, 51.2.
-uint32_t tile_tokens(uint32_t groups, uint32_t heads, uint32_t pairs, uint32_t rounds, uint32_t trig) {
-    uint32_t t = 1;
-    while (2 * t <= std::min<uint32_t>(kMaxTileTokens, groups) && 2 * t * pairs <= trig && t * heads < rounds * groups) t *= 2;
-    return t;
 }
 
 // what both directions share; returns a status
@@ -912,53 +903,6 @@ extern "C" int fpt_qk_rope(void* q_out, void* k_out, const void* q, const void* 
     });
 }
 
-namespace {
-// Tiles of the backward pass and its blocks, as many as are resident, shared out between queries and keys.  A tile takes as many
-// steps as its groups have heads, and kTileCost more (sines, addresses, a barrier); the shares are those for which the side that
-// takes longest, in whole rounds of tiles, is done first.  Measured against shares by heads alone (a tile's own cost as one
-// head): 2 x 4096 tokens of 32 + 8 heads of 128 the backward pass 55 us and 46, 3063 tokens of 12 + 4 heads of 64 with the forward
-// pass 17.0 and 15.5, 8192 tokens of 8 + 1 heads of 256 53 and 35, of 40 + 8 heads of 80 58 and 62.  The constant: 0.5 .. 3 differ
-// by less than that.
-constexpr float kTileCost = 1.5f;
-void share_blocks(QkRopeArgs& a, uint32_t groups, int64_t seq, int sm_count) {
-    const uint32_t total = uint32_t(sm_count * kBwdBlocks);
-    float cost[2] = {0.0f, 0.0f};      // of a token, then of a tile
-    for (int s = 0; s < 2; ++s) {
-        Side& d = a.side[s];
-        if (!d.heads) continue;
-        d.tile_tokens = tile_tokens(groups, d.heads, a.pairs.d, 8, kBwdTrig);
-        cost[s] = float(d.heads) + kTileCost * float(groups) / float(d.tile_tokens);
-    }
-    for (int s = 0; s < 2; ++s) {
-        Side& d = a.side[s];
-        if (!d.heads) continue;
-        // no more tokens a tile than keep every block busy
-        const float blocks = float(total) * cost[s] / (cost[0] + cost[1]);
-        while (d.tile_tokens > 1 && float(a.tokens / d.tile_tokens) < blocks) d.tile_tokens /= 2;
-        if (!reach(d.xs, seq, d.heads, d.tile_tokens) || !reach(d.gs, seq, d.heads, d.tile_tokens)) d.tile_tokens = 1u;
-        d.tiles = (a.tokens + d.tile_tokens - 1) / d.tile_tokens;
-        d.blocks = std::min(total, d.tiles);
-    }
-    Side &q = a.side[0], &k = a.side[1];
-    if (!q.heads || !k.heads) return;
-    const auto steps = [&](const Side& d) { return float((d.heads + groups / d.tile_tokens - 1) / (groups / d.tile_tokens)) + kTileCost; };
-    const float q_tile = steps(q), k_tile = steps(k);
-    const float even = (float(q.tiles) * q_tile + float(k.tiles) * k_tile) / float(total);      // time with nothing left over
-    const uint32_t most = std::max(1u, uint32_t(even / q_tile));
-    float least = 1e30f;
-    for (uint32_t rounds = most > 2 ? most - 2 : 1; rounds < most + 6; ++rounds) {
-        const uint32_t blocks = (q.tiles + rounds - 1) / rounds;
-        if (blocks >= total) continue;
-        const float time = std::max(float(rounds) * q_tile, float((k.tiles + total - blocks - 1) / (total - blocks)) * k_tile);
-        if (time < least) {
-            least = time;
-            q.blocks = blocks;
-            k.blocks = std::min(total - blocks, k.tiles);
-        }
-    }
-}
-}  // namespace
-
 extern "C" int64_t fpt_qk_norm_rope_bwd_workspace_bytes(int64_t q_heads, int64_t k_heads, int64_t head_dim) {
     if (q_heads < 0 || k_heads < 0 || q_heads + k_heads == 0 || head_dim <= 0) return 0;
     DeviceInfo dev;
@@ -1002,8 +946,11 @@ extern "C" int fpt_qk_norm_rope_bwd(void* dq, void* dk, void* dq_weight, void* d
         a.eps = eps;
         a.sin_sign = 0x80000000u;
         const uint32_t groups = uint32_t(kThreads / group_lanes(a.units));
-        share_blocks(a, groups, seq, dev.sm_count);
-        for (int s = 0; s < 2; ++s) blocks[s] = a.side[s].heads ? a.side[s].blocks : 0u;
+        share_blocks(a.side[0].share, a.side[0].heads, a.side[1].share, a.side[1].heads, a.tokens, groups, a.pairs.d,
+                     uint32_t(dev.sm_count * kBwdBlocks), [&](int s, uint32_t tile) {
+                         return reach(a.side[s].xs, seq, a.side[s].heads, tile) && reach(a.side[s].gs, seq, a.side[s].heads, tile);
+                     });
+        for (int s = 0; s < 2; ++s) blocks[s] = a.side[s].heads ? a.side[s].share.blocks : 0u;
         for (int s = 0; s < 2; ++s)
             a.side[s].partial = (s ? dk_weight : dq_weight) ? partial + (s ? int64_t(blocks[0]) * head_dim : 0) : nullptr;
         const unsigned grid = blocks[0] + blocks[1];
