@@ -19,7 +19,8 @@
 // value of q and k, once instructions and shared-memory reads are few enough: pairs are kept as two fp32 vectors (first
 // members, second members), which costs nothing to unpack, and handled by the two-wide fp32 instructions.
 // Measured, 2 x 4096 tokens x (32 + 8) heads x 128 bf16: forward with the norm 29.2 us = 5.7 TB/s, backward 46 us = 5.4 TB/s
-// (next to the memory bound by latencies at 16 warps an SM); rotation alone of 15840 such tokens 50.0 us = 6.5 TB/s.
+// (next to the memory bound by latencies at 16 warps an SM); rotation alone of 15840 such tokens 50.0 us = 6.5 TB/s.  In fp32 at the
+// first size: 77 us = 4.4 TB/s, 135 us = 3.7 TB/s, rotation alone 78 us = 4.3 TB/s.
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -38,7 +39,10 @@ constexpr int kMaxAxes = 4;
 constexpr int kStages = 3;              // items of a thread in its ring
 // Blocks an SM holds, by registers (16-bit data; 2 in fp32).  Measured: the forward pass with the norm 29.5 us at 3 and 33.3 at 4
 // (which spills), the rotation alone 51.8 at 3 and 50.8 at 4, forward and backward pass together 121 with the backward
-// pass at 3 (spills) and 87 at 2 (before the shares of share_blocks).
+// pass at 3 (spills) and 87 at 2 (before the shares of share_blocks).  The backward pass in fp32 with runs of 8 holds 96 KB of
+// rings and 18 KB besides: one block is resident and the second half of them follows.  With the sines' arrays cut to what a
+// tile uses two are resident, which is not always faster (us, one and two): 2 x 4096 tokens of 32 + 8 heads of 128 135 and 146, of
+// 8 + 1 of 256 89 and 81, of 40 + 8 of 80 134 and 124; the 16-byte copies at a stride of 32 bytes ask the L2 for every sector twice.
 template <class T, bool NORM>
 constexpr int kFwdBlocks = sizeof(T) == 4 ? 2 : NORM ? 3 : 4;
 constexpr int kBwdBlocks = 2;

@@ -22,9 +22,9 @@ struct BwdShare {                       // queries or keys in the backward pass
     uint32_t blocks, tiles, tile_tokens;
 };
 
-// Tiles of the backward pass and its blocks, `total` at most (as many as are resident, and as many as the workspace has rows for),
-// shared out between queries and keys.  A tile takes as many steps as its groups have heads, and kTileCost more (sines,
-// addresses, a barrier); the shares are those for which the side that takes longest, in whole rounds of tiles, is done first.
+// Tiles of the backward pass and its blocks, `total` at most (as many as are resident with 16-bit data, and as many as the
+// workspace has rows for), shared out between queries and keys.  A tile takes as many steps as its groups have heads, and
+// kTileCost more (sines, addresses, a barrier); the shares are those for which the side that takes longest, in whole rounds of tiles, is done first.
 // Measured against shares by heads alone (a tile's own cost as one head): 2 x 4096 tokens of 32 + 8 heads of 128 the backward pass
 // 55 us and 46, 3063 tokens of 12 + 4 heads of 64 with the forward pass 17.0 and 15.5, 8192 tokens of 8 + 1 heads of 256 53 and
 // 35, of 40 + 8 heads of 80 58 and 62.  The constant: 0.5 .. 3 differ by less than that.
