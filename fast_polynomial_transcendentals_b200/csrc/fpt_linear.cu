@@ -854,13 +854,13 @@ __global__ void __launch_bounds__(kActThreads) linear_grad_act_kernel(const Grad
     __shared__ float sums[kActRowLanes][kActColumns + 1];
     const int lane = threadIdx.x & 31, row_lane = threadIdx.x >> 5;
     const int column = blockIdx.x * kActColumns + 8 * lane;
-    const int row_end = min(p.rows, (int(blockIdx.y) + 1) * p.chunk_rows);
+    const int row_first = int(blockIdx.y) * p.chunk_rows, row_end = row_first + min(p.chunk_rows, p.rows - row_first);   // not past 2^31
     const int live = min(8, p.out - column);                    // columns of this lane that exist
     wait_for_inputs();
     float sum[8] = {};
     if (live > 0) {
 #pragma unroll 2
-        for (int row = int(blockIdx.y) * p.chunk_rows + row_lane; row < row_end; row += kActRowLanes) {
+        for (int row = row_first + row_lane; row < row_end; row += kActRowLanes) {
             const uint16_t* dy = p.dy + int64_t(row) * p.dy_ld + column;
             uint32_t g[4] = {0, 0, 0, 0}, s[4] = {0, 0, 0, 0};
             if (p.vec_dy && live == 8) {

@@ -475,3 +475,16 @@ def test_small_slopes_keep_their_precision(cuda, activation, low, high, dtype, r
     exponential = (2 * z * z if activation == "gelu" else 4 * z.abs()) + 16
     slack = (2.0 ** -11 + exponential * U) * want.abs() + 2.0 ** -40 * d.abs()
     assert ((dx.double() - want).abs() <= rel * (want.abs() + slack) + slack + least).all()
+
+
+def test_column_sums_of_nearly_2_31_rows(cuda, fpt):
+    """The last block's rows would end past 31 bits (740 chunks of 2902005 rows): they count all the same."""
+    rows = 2 ** 31 - 300
+    dy = torch.zeros(rows, 1, dtype=torch.bfloat16, device=cuda)
+    dy[0], dy[rows // 2], dy[-1] = 1, 2, 4
+    lib, db = fpt.load(), torch.empty(1, device=cuda)
+    nbytes = lib.fpt_linear_grad_act_workspace_bytes(rows, 1)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=cuda)
+    fpt.call("fpt_linear_grad_act", None, db.data_ptr(), dy.data_ptr(), None, workspace.data_ptr(), nbytes, rows, 1, 8, 1, 8, 1, 2,
+             torch.cuda.current_stream().cuda_stream)
+    assert db.item() == 7
