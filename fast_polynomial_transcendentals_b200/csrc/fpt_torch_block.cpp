@@ -19,6 +19,7 @@
 #include <torch/library.h>
 
 #include <cmath>
+#include <cstring>
 #include <memory>
 #include <mutex>
 #include <string>
@@ -349,28 +350,31 @@ std::tuple<Tensor, Tensor> qk_rope_autograd(const Tensor& q, const Tensor& k, co
 // ---- fpt_linear -----------------------------------------------------------------------------------------------------
 
 // The word a bounded device-side wait reports to: mapped host memory, so that a call looks at it without a copy or an
-// event.  One for the process, made at the first call (also inside a stream capture, where plain allocation is an error).
-volatile uint32_t* status_word() {
-    static uint32_t* word = [] {
+// event.  One for each device, made together at the first call (also inside a stream capture, where plain allocation is an
+// error).
+constexpr int kMaxDevices = 64, kStatusBytes = 64;
+volatile uint32_t* status_word(int64_t device) {
+    static char* words = [] {
         cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
         cudaThreadExchangeStreamCaptureMode(&mode);
         void* p = nullptr;
-        const cudaError_t e = cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped);
+        const cudaError_t e = cudaHostAlloc(&p, kMaxDevices * kStatusBytes, cudaHostAllocPortable | cudaHostAllocMapped);
         cudaThreadExchangeStreamCaptureMode(&mode);
-        TORCH_CHECK(e == cudaSuccess, "no host memory for the status word: ", cudaGetErrorString(e));
-        *static_cast<uint32_t*>(p) = 0;
-        return static_cast<uint32_t*>(p);
+        TORCH_CHECK(e == cudaSuccess, "no host memory for the status words: ", cudaGetErrorString(e));
+        std::memset(p, 0, kMaxDevices * kStatusBytes);
+        return static_cast<char*>(p);
     }();
-    return word;
+    TORCH_CHECK(device >= 0 && device < kMaxDevices, "no status word for device ", device);
+    return reinterpret_cast<uint32_t*>(words + device * kStatusBytes);
 }
 
-void poll_linear_status() {
-    volatile uint32_t* word = status_word();
+void poll_linear_status(int64_t device) {
+    volatile uint32_t* word = status_word(device);
     const uint32_t value = *word;
     if (value) {
         *word = 0;
         TORCH_CHECK(false, fpt_status_string(FPT_ERR_DEVICE_TIMEOUT), ": status word ", value, " (waiting point ", value & 0xffff,
-                    ") left by an earlier linear_act; the outputs of that call are invalid");
+                    ") left by an earlier linear_act on cuda:", device, "; the outputs of that call are invalid");
     }
 }
 
@@ -425,8 +429,8 @@ Tensor as_operand(const Tensor& t, int64_t rows, int64_t columns) {
 std::tuple<Tensor, Tensor> run_linear(const Tensor& x_in, const Tensor& weight_in, const OptTensor& bias_in, const OptTensor& residual_in,
                                       int64_t function, int64_t degree, int64_t source, bool want_slope) {
     const Linear l = check_linear(x_in, weight_in, bias_in, residual_in, function, degree, source);
-    poll_linear_status();
     const c10::cuda::CUDAGuard guard(x_in.device());
+    poll_linear_status(x_in.device().index());
     Tensor out = at::empty(l.shape, x_in.options(), at::MemoryFormat::Contiguous);
     const int64_t padded = (l.out + 7) / 8 * 8;
     Tensor slope = at::empty({want_slope && function != FPT_FN_NONE ? l.rows : 0, padded}, x_in.options().dtype(at::kHalf), at::MemoryFormat::Contiguous);
@@ -438,7 +442,7 @@ std::tuple<Tensor, Tensor> run_linear(const Tensor& x_in, const Tensor& weight_i
                               bias.defined() ? bias.data_ptr() : nullptr, residual.defined() ? residual.data_ptr() : nullptr, l.rows,
                               l.dim, l.out, row_stride(x), row_stride(weight), l.out, residual.defined() ? row_stride(residual) : 0,
                               padded, dtype_id(x.scalar_type()), bias.defined() ? dtype_id(bias.scalar_type()) : FPT_FP32,
-                              int(function), int(degree), int(source), const_cast<uint32_t*>(status_word()), stream_of(x));
+                              int(function), int(degree), int(source), const_cast<uint32_t*>(status_word(x.device().index())), stream_of(x));
     TORCH_CHECK(rc != FPT_ERR_UNKNOWN_PROGRAM, "Unsupported activation degree: ", degree);
     check_status(rc, "fpt_linear");
     return {out, slope};
@@ -474,8 +478,8 @@ std::tuple<Tensor, Tensor, Tensor> linear_act_bwd(const Tensor& dy_in, const Ten
             TORCH_CHECK((*t)->scalar_type() == dy_in.scalar_type() && (*t)->device() == dy_in.device(), "x and weight must have the gradient's dtype and device");
     TORCH_CHECK(!want_x || (weight_in->dim() == 2 && weight_in->size(0) == out && weight_in->size(1) == dim), "the weight does not fit the gradient");
     TORCH_CHECK(!want_weight || x_in->sizes() == x_shape, "x does not fit the gradient");
-    poll_linear_status();
     const c10::cuda::CUDAGuard guard(dy_in.device());
+    poll_linear_status(dy_in.device().index());
     const int dtype = dtype_id(dy_in.scalar_type());
     Tensor dx = at::empty(want_x ? x_shape : at::IntArrayRef({0}), dy_in.options(), at::MemoryFormat::Contiguous);
     Tensor dw = at::empty({want_weight ? out : 0, dim}, dy_in.options(), at::MemoryFormat::Contiguous);
@@ -493,7 +497,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_act_bwd(const Tensor& dy_in, const Ten
                                          padded, rows ? row_stride(dy) : out, padded, dtype, int(bias_dtype), stream_of(dy)),
                      "fpt_linear_grad_act");
     }
-    void* status = const_cast<uint32_t*>(status_word());
+    void* status = const_cast<uint32_t*>(status_word(dy_in.device().index()));
     const int64_t dz_ld = copy ? padded : rows ? row_stride(dz) : padded;
     if (want_x && rows) {
         const Tensor weight = as_operand(*weight_in, out, dim);
@@ -661,4 +665,5 @@ void register_block_operators(pybind11::module_& m) {
     m.def("qk_rope", &enter_qk_rope);
     m.def("linear_act", &enter_linear);
     m.def("poll_linear_status", &poll_linear_status);
+    m.def("linear_status_address", [](int64_t device) { return reinterpret_cast<uintptr_t>(status_word(device)); });
 }

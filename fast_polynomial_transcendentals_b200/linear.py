@@ -41,10 +41,12 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
 
 
 def check_linear_status(device=None) -> None:
-    """Wait for the work on `device` (default: the current one) and raise RuntimeError if a `linear_act` reported a
-    device-side wait that ran out.  Without this call the same error surfaces, without blocking, at the next `linear_act`."""
+    """Wait for the work on `device` (default: the current one) and raise RuntimeError if a `linear_act` on it reported a
+    device-side wait that ran out.  Without this call the same error surfaces, without blocking, at the next `linear_act` on
+    that device, from whichever thread, and is cleared there."""
     torch.cuda.synchronize(device)
-    _ext.poll_linear_status()
+    index = None if device is None else torch.device(device).index
+    _ext.poll_linear_status(torch.cuda.current_device() if index is None else index)
 
 
 @torch.library.register_fake("fpt_b200::linear_act")

@@ -488,3 +488,28 @@ def test_column_sums_of_nearly_2_31_rows(cuda, fpt):
     fpt.call("fpt_linear_grad_act", None, db.data_ptr(), dy.data_ptr(), None, workspace.data_ptr(), nbytes, rows, 1, 8, 1, 8, 1, 2,
              torch.cuda.current_stream().cuda_stream)
     assert db.item() == 7
+
+
+def test_a_reported_wait_belongs_to_its_device(cuda):
+    """A status word that the host writes as a kernel would: the next call on that device raises, once; another device's word is
+    left for calls there."""
+    import ctypes
+    from fast_polynomial_transcendentals_b200 import _fpt_torch
+    x, w, b, _, _ = inputs(4, 64, 24, torch.bfloat16, cuda)
+    want = linear_act(x, w, b)
+    check_linear_status()
+    words = [ctypes.c_uint32.from_address(_fpt_torch.linear_status_address(i)) for i in (0, 1)]
+    words[1].value = 0x80000052
+    assert torch.equal(linear_act(x, w, b), want)
+    check_linear_status(cuda)
+    with pytest.raises(RuntimeError, match="cuda:1"):
+        _fpt_torch.poll_linear_status(1)
+    assert words[1].value == 0
+    words[0].value = 0x80000052
+    with pytest.raises(RuntimeError, match="cuda:0"):
+        linear_act(x, w, b)
+    assert words[0].value == 0 and torch.equal(linear_act(x, w, b), want)
+    words[0].value = 0x80000053
+    with pytest.raises(RuntimeError, match="cuda:0"):
+        check_linear_status(0)
+    check_linear_status("cuda")
