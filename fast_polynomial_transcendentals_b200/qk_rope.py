@@ -73,8 +73,9 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor, phase_increments: torch.Tensor, 
     positions: int32 or int64, `[axes, S]` or `[axes, B, S]` (or `[axes, 1, S]`), one to four axes.  sections: how many
     pairs each axis has; they add up to the entries of phase_increments, which hold one increment per pair whatever its
     axis (`sfu_repro.rope.rope_axis_phase_increments` starts the frequencies anew in every section).  section_order:
-    "blocked" gives the first `sections[0]` pairs to axis 0 and so on, "cyclic" deals the pairs out in turn until an
-    axis has its share.  pairing as in `qk_norm_rope`.  Gradients: q and k."""
+    "blocked" gives the first `sections[0]` pairs to axis 0 and so on.  "cyclic" deals the pairs out in turn until an axis has
+    its share, and goes on among the others: [2, 3, 3] is 0 1 2 0 1 2 1 2.  A model that interleaves its axes and leaves every
+    pair that is over to axis 0 means the same only where the other sections are equal and the first is not smaller.  pairing as in `qk_norm_rope`.  Gradients: q and k."""
     if sections is None or len(sections) == 0 or positions is None:
         raise RuntimeError("rope_axes needs sections and positions")
     return _call(q, k, None, None, phase_increments, positions, list(sections), _choice(_ORDERS, section_order, "section_order"),
