@@ -151,7 +151,7 @@ Rope check_rope(const Tensor& q, const Tensor& k, const OptTensor& q_weight, con
             r.weight_dtype = dtype_id((*w)->scalar_type());
         }
     TORCH_CHECK(!q_weight || !k_weight || q_weight->scalar_type() == k_weight->scalar_type(), "q_weight and k_weight must have the same dtype");
-    TORCH_CHECK(!norm || (eps >= 0 && std::isfinite(eps)), "eps must be finite and not negative");
+    TORCH_CHECK(!norm || (eps >= 0 && std::isfinite(float(eps))), "eps must be finite in fp32 and not negative");
     if (!sections.empty()) {
         TORCH_CHECK(positions.has_value(), "sections go with positions of one row per axis");
         TORCH_CHECK(int64_t(sections.size()) <= kMaxAxes, "at most ", kMaxAxes, " sections");

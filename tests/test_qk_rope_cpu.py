@@ -105,3 +105,8 @@ def test_increments_start_anew_in_every_section():
     assert inc.dtype == torch.int32 and inc.numel() == 14
     assert torch.equal(inc[4:12], rope_phase_increments(16, theta=100.0))
     assert inc[0] == inc[4] == inc[12] == round(2 ** 32 / (2 * math.pi))
+
+
+def test_eps_beyond_fp32_is_refused():
+    with pytest.raises(RuntimeError, match="finite"):
+        qk_rope.qk_norm_rope(heads(), heads(), None, None, INC, eps=1e39)
