@@ -294,13 +294,14 @@ def _other_than_two_layers(module: nn.Module, pair: tuple[str, str], slot: str) 
     if getattr(own, "__func__", None) is not type(module).forward:
         return "a forward of its own"
     for training in (True, False):
-        x, hidden, active, y = (torch.zeros(2, 3, n) for n in (up.in_features, up.out_features, down.in_features, down.out_features))
+        x, hidden, active, y = (torch.zeros(2, 3, n, device="cpu")
+                                for n in (up.in_features, up.out_features, down.in_features, down.out_features))
         steps = {pair[0]: _Step(x, hidden), slot: _Step(hidden, active), pair[1]: _Step(active, y)}
-        probe = copy.copy(module)
-        probe.__dict__["_modules"] = {**module._modules, **{n: s for n, s in steps.items() if n in module._modules}}
-        probe.__dict__.update({n: s for n, s in steps.items() if n not in module._modules})
-        probe.__dict__["training"] = training
         try:
+            probe = copy.copy(module)
+            probe.__dict__["_modules"] = {**module._modules, **{n: s for n, s in steps.items() if n in module._modules}}
+            probe.__dict__.update({n: s for n, s in steps.items() if n not in module._modules})
+            probe.__dict__["training"] = training
             with torch.no_grad(), torch.random.fork_rng(devices=[]):
                 result = type(module).forward(probe, x)
         except Exception as error:

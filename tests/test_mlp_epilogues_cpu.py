@@ -180,3 +180,12 @@ def test_a_dropout_that_begins_to_drop_is_not_lost(as_on_the_gpu):
         change(model)
         model(torch.randn(3, 16))
         assert calls == [1]
+
+
+def test_a_module_that_cannot_be_copied_is_left_alone():
+    class Alone(Mlp):
+        def __copy__(self):
+            raise TypeError("there is one of it")
+
+    model, skipped = Alone(), []
+    assert adapters.patch_mlp_epilogues(model, skipped=skipped) == 0 and "there is one of it" in skipped[0][1]
